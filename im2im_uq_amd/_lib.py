@@ -122,6 +122,16 @@ SIGNATURES = {
     "im2im_complex_transpose": (_i32, [_ptr, _ptr, _i32, _i32, _i32, _i32, _i32, _ptr]),
     "im2im_fastmri_abs_normalize": (_i32, [_ptr, _ptr, _i32, _i32, _i32, _i32, _f32, _f32, _ptr]),
     "im2im_center_crop_affine": (_i32, [_ptr, _ptr, _i64, _i32, _i32, _i32, _i32, _f32, _f32, _ptr]),
+    "im2im_relpos_line_len": (_i64, [_i32, _i32]),
+    "im2im_relpos_line": (_i32, [_ptr, _i32, _i32, _i32, _ptr, _ptr, _i32, _i32, _ptr, _ptr]),
+    "im2im_attention_fwd_workspace_bytes": (_i64, [_ptr]),
+    "im2im_attention_fwd": (_i32, [_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "im2im_attention_bwd_workspace_bytes": (_i64, [_ptr, _i32]),
+    "im2im_attention_bwd": (_i32, [_ptr, _ptr, _ptr, _i64, _ptr]),
+    "im2im_norm_gate_fwd": (_i32, [_ptr, _ptr, _ptr, _ptr]),
+    "im2im_norm_gate_bwd_workspace_bytes": (_i64, [_i64, _i32]),
+    # desc, dy, dh, dx, df, dgate, dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias, ws, ws_bytes, stream
+    "im2im_norm_gate_bwd": (_i32, [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
     "im2im_adam_step": (_i32, [_i32, _ptr, _ptr, _ptr, _ptr, _ptr, _f32, _f32, _f32, _f32, _i64, _ptr]),
     "im2im_adam_step_dev": (_i32, [_i32, _ptr, _ptr, _ptr, _ptr, _ptr, _f32, _f32, _f32, _f32, _ptr, _ptr, _ptr]),
 }
@@ -129,6 +139,26 @@ for _name, (_res, _args) in SIGNATURES.items():
     _fn = getattr(lib, _name)
     _fn.restype = _res
     _fn.argtypes = _args
+
+
+class AttentionDesc(ctypes.Structure):
+    """im2im_attention_desc"""
+    _fields_ = [("q", _ptr), ("k", _ptr), ("v", _ptr), ("line", _ptr), ("lengths", _ptr), ("lam", _ptr), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3),
+                ("v_stride", _i64 * 3), ("B", _i32), ("Lq", _i32), ("Lk", _i32), ("H", _i32), ("D", _i32), ("maps", _i32), ("gh", _i32), ("gw", _i32),
+                ("q_start", _i32), ("dtype", _i32), ("scale", _f32)]
+
+
+class AttentionGrads(ctypes.Structure):
+    """im2im_attention_grads"""
+    _fields_ = [("dout", _ptr), ("lse", _ptr), ("map_out", _ptr), ("dq", _ptr), ("dk", _ptr), ("dv", _ptr), ("dtable", _ptr), ("dlam", _ptr),
+                ("thr_y", _ptr), ("thr_x", _ptr), ("dq_stride", _i64 * 3), ("dk_stride", _i64 * 3), ("dv_stride", _i64 * 3), ("ny", _i32), ("nx", _i32)]
+
+
+class NormGateDesc(ctypes.Structure):
+    """im2im_norm_gate_desc"""
+    _fields_ = [("x", _ptr), ("f", _ptr), ("gate", _ptr), ("scale", _ptr), ("post_weight", _ptr), ("post_bias", _ptr), ("pre_weight", _ptr),
+                ("pre_bias", _ptr), ("rows", _i64), ("x_stride", _i64), ("f_stride", _i64), ("gate_stride", _i64), ("C", _i32), ("norm", _i32),
+                ("dtype", _i32), ("eps", _f32)]
 
 
 def check(rc: int, what: str) -> None:

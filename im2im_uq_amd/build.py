@@ -20,8 +20,8 @@ LIB = os.path.join(PKG, "lib", "libim2im_uq.so")
 ARCH = "gfx950"
 
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-result"]
-# [r6] compiles a file without any packed fp32 instruction (the host pass prints "not a recognized feature": expected).  Not used by default:
-# the BatchNorm kernels of elementwise.hip lose 1.1 % of the step without v_pk_* (37.44 -> 37.90 ms, same box, alternating) -- the unreliable
+# [r6] compiles a file without any packed fp32 instruction (the host pass prints "not a recognized feature": expected).  The files of the
+# attention bottleneck are compiled so.  Not the others: the BatchNorm kernels of elementwise.hip lose 1.1 % of the step without v_pk_* (37.44 -> 37.90 ms, same box, alternating) -- the unreliable
 # op_sel forms (profiles/r06_multiprocess_determinism.txt) are kept out at their sources and by tests/test_abi.py's scan of the built library
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-source extra flags.  rcps.hip: the reference's CPU path never fuses mul+add.
@@ -37,6 +37,9 @@ SOURCES = {
     "smallconv.hip": ["-ffp-contract=off"],
     "fastmri.hip": ["-ffp-contract=off"],
     "conv_fp8.hip": ["-ffp-contract=off"],
+    "attention_fwd.hip": NO_PACKED_FP32,
+    "attention_bwd.hip": NO_PACKED_FP32,
+    "token_norm.hip": NO_PACKED_FP32,
 }
 
 

@@ -1,0 +1,497 @@
+// Grid attention, backward.  With P_m the softmax maps, A = P_1 (- lam P_2) and dP = dO V^T:
+//   dV = A^T dO,   dS_1 = P_1 o (dP - D_1),   dS_2 = P_2 o (-lam dP - D_2),   D_m = rowsum(P_m o dP_m) = dO . O_m (times -lam for m = 2),
+//   dQ_m = scale dS_m K_m,   dK_m = scale dS_m^T Q_m,   dbias(j - i) = sum of dS_1 + dS_2,   dlam = -sum P_2 o dP.
+// Two passes, each with its own tile of the scores (computed again from Q, K and the saved log-sums): queries' gradients and the bias in
+// one, keys' and values' gradients in the other.  No global atomics: every sum has one order.
+#include "attention_common.h"
+
+namespace im2im {
+
+// D of every row, 16 lanes a row: reads dO and the saved map results once (bound by that)
+template <typename T, int MAPS> __global__ __launch_bounds__(256) void attn_delta_kernel(const AttnArgs a, float* delta) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row >= rows) return;
+  const int i = (int)(row % a.Lq), bh = (int)(row / a.Lq), h = bh % a.H, b = bh / a.H, l = threadIdx.x & 15;
+  const T* g = static_cast<const T*>(a.dout) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv;
+  float acc[MAPS] = {};
+  for (int c = l * 4; c < a.dv; c += 64) {
+    float gv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) gv[e] = to_float(g[c + e]);
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.osave + (row * MAPS + m) * a.dv + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m] = fmaf(gv[e], x[e], acc[m]);
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+#pragma unroll
+    for (int s = 8; s >= 1; s >>= 1) acc[m] += __shfl_xor(acc[m], s);
+    if (l == 0) delta[((int64_t)bh * MAPS + m) * a.Lq + i] = m == 0 ? acc[m] : -a.lam[h] * acc[m];
+  }
+}
+
+// -------------------------------------------------------------------------------------- queries' gradients, bias and lam
+// One workgroup: 128 queries of one head, of `group_images` images in turn, against their keys in tiles of 64.
+// Bias gradient: a pair's place in the line is code(j) - code(i) + off.  Within one instruction 32 lanes have 32 different queries and the
+// same key, so their places differ; the other 32 lanes have another key and add to a copy of their own; each wave has its own pair
+// of copies and its additions are in program order: no order is left open.  A copy is a ring over the line's index: the places
+// that the following tiles cannot reach any more are summed over the copies and written, each once (bias gradient = one LDS addition a
+// pair, and 2 gw + 128 floats a tile).
+template <typename T, int DQ, int DV, int MAPS, bool BIAS>
+__global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* Ks = reinterpret_cast<T*>(smem);
+  T* Vs = Ks + MAPS * KEYS * SQ;
+  int* kc = reinterpret_cast<int*>(Vs + KEYS * SV);
+  float* red = reinterpret_cast<float*>(kc + KEYS);              // [WAVES]
+  float* ring = red + 64;                                        // [2 * WAVES][a.ring]
+  float* win = ring + (BIAS ? 2 * WAVES * a.ring : 0);
+
+  const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, gh_ = lin / a.nq, h = gh_ % a.H, group = gh_ / a.H;
+  const int slot = group * a.nq + qt;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int i0 = qt * ROWS, i_last = min(i0 + ROWS, a.Lq) - 1;
+  const int i = i0 + wave * 32 + (lane & 31), ic = min(i, i_last);
+  const bool mine = i < a.Lq, busy = i0 + wave * 32 < a.Lq;
+  const int code_last = grid_code(a.q_start + i_last, a.gw);
+  const int aoff = code_last - grid_code(a.q_start + ic, a.gw);
+  const int qspan = code_last - grid_code(a.q_start + i0, a.gw);
+  const float scale2 = a.scale * LOG2E, lam = MAPS == 2 ? a.lam[h] : 0.f;
+  const float* line = a.line + (int64_t)h * a.line_len;
+  const int mask = a.ring - 1;
+  float* my_ring = ring + (wave * 2 + half) * a.ring;
+  float* line_out = BIAS ? a.line_part + ((int64_t)slot * a.H + h) * a.line_len : nullptr;
+  const int line_begin = a.line_off - code_last, line_end = grid_code(a.Lk - 1, a.gw) - code_last + a.line_off + qspan + 1;
+  float dlam = 0.f;
+
+  if (BIAS)
+    for (int w = threadIdx.x; w < 2 * WAVES * a.ring; w += 64 * WAVES) ring[w] = 0.f;
+
+  const int b0 = group * a.group_images, b1 = min(b0 + a.group_images, a.B);
+  for (int b = b0; b < b1; ++b) {
+    const int64_t bh = (int64_t)b * a.H + h;
+    Frag qf[MAPS][DQ / M::KC], gf[DV / M::KC];
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+      load_row_frags<T, DQ>(qf[m], static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)ic * a.qs[1] + (int64_t)(MAPS * h + m) * a.qs[2], mine,
+                            a.d, half);
+    load_row_frags<T, DV>(gf, static_cast<const T*>(a.dout) + (((int64_t)b * a.Lq + ic) * a.H + h) * a.dv, mine, a.dv, half);
+    float lse[MAPS], del[MAPS];
+    f32x16 acc[MAPS][DQ / 32];
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      lse[m] = mine ? a.lse[(bh * MAPS + m) * a.Lq + ic] : INFINITY;
+      del[m] = mine ? a.delta[(bh * MAPS + m) * a.Lq + ic] : 0.f;
+#pragma unroll
+      for (int n = 0; n < DQ / 32; ++n) acc[m][n] = zero16();
+    }
+    const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
+    const int tiles = (len + KEYS - 1) / KEYS;
+    const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)(MAPS * h) * a.ks[2];
+    const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
+    int done = line_begin;                                       // line places that are written
+
+    for (int t = 0; t < tiles; ++t) {
+      const int j0 = t * KEYS, valid = min(len - j0, KEYS);
+      const int kfirst = grid_code(j0, a.gw), base = kfirst - code_last + a.line_off;
+      const int wlen = grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1;
+      __syncthreads();
+      if (BIAS) {                                                // a place's thread is the same for every image
+        for (int w = done + ((int)threadIdx.x - done & 255); w < base; w += 64 * WAVES) {
+          float s = 0.f;
+#pragma unroll
+          for (int c = 0; c < 2 * WAVES; ++c) {
+            s += ring[c * a.ring + (w & mask)];
+            ring[c * a.ring + (w & mask)] = 0.f;
+          }
+          line_out[w] = b == b0 ? s : line_out[w] + s;
+        }
+        done = base;
+      }
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Ks + m * KEYS * SQ, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
+      stage_rows<T, DV, KEYS>(Vs, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+      if (threadIdx.x < KEYS) kc[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
+      for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
+      __syncthreads();
+      if (!busy) continue;
+
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        f32x16 dp = zero16(), s[MAPS];
+#pragma unroll
+        for (int c = 0; c < DV / M::KC; ++c)
+          dp = M::mma(load_frag<T>(Vs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), gf[c], dp);
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          s[m] = zero16();
+#pragma unroll
+          for (int c = 0; c < DQ / M::KC; ++c)
+            s[m] = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], s[m]);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = sub * 32 + mfma_row(r, half), w = kc[j] + aoff;
+          const float bias = win[w];
+          float ds[MAPS], total = 0.f;
+#pragma unroll
+          for (int m = 0; m < MAPS; ++m) {
+            float p = exp2_(fmaf(s[m][r], scale2, bias) - lse[m]);
+            p = j < valid ? p : 0.f;
+            if (m == 1) dlam = fmaf(p, dp[r], dlam);
+            ds[m] = p * ((m == 0 ? dp[r] : -lam * dp[r]) - del[m]);
+            s[m][r] = ds[m];
+            total += ds[m];
+          }
+          if (BIAS) __hip_atomic_fetch_add(my_ring + (base + w & mask), total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 32 / M::KC; ++ks)
+#pragma unroll
+          for (int m = 0; m < MAPS; ++m) {
+            const Frag df = M::pack(s[m], ks);
+#pragma unroll
+            for (int n = 0; n < DQ / 32; ++n) acc[m][n] = M::mma(M::load_t(Ks + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, acc[m][n]);
+          }
+      }
+    }
+
+    if (BIAS) {
+      __syncthreads();
+      for (int w = done + ((int)threadIdx.x - done & 255); w < line_end; w += 64 * WAVES) {
+        float s = 0.f;
+        if (w - done < a.ring) {
+#pragma unroll
+          for (int c = 0; c < 2 * WAVES; ++c) {
+            s += ring[c * a.ring + (w & mask)];
+            ring[c * a.ring + (w & mask)] = 0.f;
+          }
+        }
+        line_out[w] = b == b0 ? s : line_out[w] + s;
+      }
+    }
+    if (mine) {
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        T* dst = static_cast<T*>(a.dq) + b * a.dqs[0] + (int64_t)i * a.dqs[1] + (int64_t)(MAPS * h + m) * a.dqs[2];
+#pragma unroll
+        for (int n = 0; n < DQ / 32; ++n)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int c = n * 32 + 8 * g + 4 * half;
+            if (c < a.d)
+              store4(dst + c, acc[m][n][4 * g] * a.scale, acc[m][n][4 * g + 1] * a.scale, acc[m][n][4 * g + 2] * a.scale, acc[m][n][4 * g + 3] * a.scale);
+          }
+      }
+    }
+  }
+  if (MAPS == 2) {
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) dlam += __shfl_xor(dlam, s);
+    __syncthreads();
+    if (lane == 0) red[wave] = dlam;
+    __syncthreads();
+    if (threadIdx.x == 0) a.dlam_part[(int64_t)slot * a.H + h] = -(red[0] + red[1] + red[2] + red[3]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- keys' and values' gradients
+// One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.
+template <typename T, int DQ, int DV, int MAPS>
+__global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* Qs = reinterpret_cast<T*>(smem);
+  T* Gs = Qs + MAPS * KEYS * SQ;
+  int* qc = reinterpret_cast<int*>(Gs + KEYS * SV);
+  float* rows = reinterpret_cast<float*>(qc + KEYS);             // [2][MAPS][KEYS]: log-sums, D
+  float* win = rows + 2 * MAPS * KEYS;
+
+  const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
+  const int k0 = kt * ROWS, k_last = min(k0 + ROWS, a.Lk) - 1;
+  const int j = k0 + wave * 32 + (lane & 31), jc = min(j, k_last);
+  const bool mine = j < len, busy = k0 + wave * 32 < len;
+  const int code_first = grid_code(k0, a.gw), koff = grid_code(jc, a.gw) - code_first, kspan = grid_code(k_last, a.gw) - code_first;
+  const float scale2 = a.scale * LOG2E, lam = MAPS == 2 ? a.lam[h] : 0.f;
+  const float* line = a.line + (int64_t)h * a.line_len;
+
+  Frag kf[MAPS][DQ / M::KC], vf[DV / M::KC];
+  f32x16 dk[MAPS][DQ / 32], dv[DV / 32];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    load_row_frags<T, DQ>(kf[m], static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)jc * a.ks[1] + (int64_t)(MAPS * h + m) * a.ks[2], mine, a.d,
+                          half);
+#pragma unroll
+    for (int n = 0; n < DQ / 32; ++n) dk[m][n] = zero16();
+  }
+  load_row_frags<T, DV>(vf, static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)jc * a.vs[1] + (int64_t)h * a.vs[2], mine, a.dv, half);
+#pragma unroll
+  for (int n = 0; n < DV / 32; ++n) dv[n] = zero16();
+
+  const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(MAPS * h) * a.qs[2];
+  const T* gp = static_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * a.dv;
+  const int tiles = k0 < len ? (a.Lq + KEYS - 1) / KEYS : 0;
+  for (int t = 0; t < tiles; ++t) {
+    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS);
+    const int code_last = grid_code(a.q_start + i0 + valid - 1, a.gw), base = code_first - code_last + a.line_off;
+    const int wlen = code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Qs + m * KEYS * SQ, qp + (int64_t)i0 * a.qs[1] + m * a.qs[2], a.qs[1], valid, a.d);
+    stage_rows<T, DV, KEYS>(Gs, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, valid, a.dv);
+    if (threadIdx.x < KEYS) {
+      const int i = min((int)threadIdx.x, valid - 1);
+      qc[threadIdx.x] = code_last - grid_code(a.q_start + i0 + i, a.gw);
+    }
+    for (int w = threadIdx.x; w < MAPS * KEYS; w += 64 * WAVES) {
+      const int m = w / KEYS, i = w % KEYS;
+      const int64_t at = ((int64_t)bh * MAPS + m) * a.Lq + i0 + i;
+      rows[w] = i < valid ? a.lse[at] : INFINITY;                // behind the last query: probabilities of zero
+      rows[MAPS * KEYS + w] = i < valid ? a.delta[at] : 0.f;
+    }
+    for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
+    __syncthreads();
+    if (!busy) continue;
+
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 dp = zero16(), s[MAPS], mix;
+#pragma unroll
+      for (int c = 0; c < DV / M::KC; ++c)
+        dp = M::mma(load_frag<T>(Gs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), vf[c], dp);
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        s[m] = zero16();
+#pragma unroll
+        for (int c = 0; c < DQ / M::KC; ++c)
+          s[m] = M::mma(load_frag<T>(Qs + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), kf[m][c], s[m]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = sub * 32 + mfma_row(r, half);
+        const float bias = win[qc[i] + koff];
+        float sum = 0.f;
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          float p = exp2_(fmaf(s[m][r], scale2, bias) - rows[m * KEYS + i]);
+          p = mine ? p : 0.f;
+          sum = m == 0 ? p : fmaf(-lam, p, sum);
+          s[m][r] = p * ((m == 0 ? dp[r] : -lam * dp[r]) - rows[(MAPS + m) * KEYS + i]);
+        }
+        mix[r] = sum;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 32 / M::KC; ++ks) {
+        const Frag pf = M::pack(mix, ks);
+#pragma unroll
+        for (int n = 0; n < DV / 32; ++n) dv[n] = M::mma(M::load_t(Gs, SV, sub * 32, ks, n * 32), pf, dv[n]);
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          const Frag df = M::pack(s[m], ks);
+#pragma unroll
+          for (int n = 0; n < DQ / 32; ++n) dk[m][n] = M::mma(M::load_t(Qs + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, dk[m][n]);
+        }
+      }
+    }
+  }
+  if (j >= a.Lk) return;                                          // keys from lengths[b] on get zeros
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    T* dst = static_cast<T*>(a.dk) + b * a.dks[0] + (int64_t)j * a.dks[1] + (int64_t)(MAPS * h + m) * a.dks[2];
+#pragma unroll
+    for (int n = 0; n < DQ / 32; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = n * 32 + 8 * g + 4 * half;
+        if (c < a.d) store4(dst + c, dk[m][n][4 * g] * a.scale, dk[m][n][4 * g + 1] * a.scale, dk[m][n][4 * g + 2] * a.scale, dk[m][n][4 * g + 3] * a.scale);
+      }
+  }
+  T* dst = static_cast<T*>(a.dvv) + b * a.dvs[0] + (int64_t)j * a.dvs[1] + (int64_t)h * a.dvs[2];
+#pragma unroll
+  for (int n = 0; n < DV / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = n * 32 + 8 * g + 4 * half;
+      if (c < a.dv) store4(dst + c, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ joining the parts
+// line[h][x] = sum over the slots whose queries reach x; 64 places a workgroup, four slots at a time
+__global__ __launch_bounds__(256) void attn_line_sum_kernel(const AttnArgs a, double* sum) {
+  __shared__ double part[4][64];
+  const int x = blockIdx.x * 64 + (threadIdx.x & 63), h = blockIdx.y, wave = threadIdx.x >> 6;
+  double acc = 0.0;
+  if (x < a.line_len)
+    for (int qt = 0; qt < a.nq; ++qt) {
+      const int first = grid_code(a.q_start + qt * ROWS, a.gw), last = grid_code(a.q_start + min(qt * ROWS + ROWS, a.Lq) - 1, a.gw);
+      if (x < a.line_off - last || x > grid_code(a.Lk - 1, a.gw) - first + a.line_off) continue;
+      for (int g = wave; g < a.groups; g += 4) acc += (double)a.line_part[((int64_t)(g * a.nq + qt) * a.H + h) * a.line_len + x];
+    }
+  part[wave][threadIdx.x & 63] = acc;
+  __syncthreads();
+  if (wave == 0 && x < a.line_len) sum[(int64_t)h * a.line_len + x] = part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+}
+
+struct BucketArgs {
+  const double* line;    // [H][line_len] or null
+  const float* dlam_part;
+  float *dtable, *dlam;
+  int ny, nx, H, gh, gw, slots;
+  int thr_y[32], thr_x[32];
+};
+
+// distances key - query of a bucket: they are consecutive, [lo, hi) clipped to the grid
+__device__ __forceinline__ void bucket_range(int b, int n, int size, const int* thr, int& lo, int& hi) {
+  const int far = size - 1;
+  if (n == 1) { lo = -far; hi = far + 1; return; }
+  const int side = n / 2, m = b % side;
+  const int from = m == 0 ? 0 : thr[m - 1], to = m + 1 < side ? thr[m] : size;      // distances [from, to)
+  if (b >= side) { lo = from < 1 ? 1 : from; hi = to < size ? to : size; }
+  else { lo = -(to < size ? to : size) + 1; hi = -from + 1; }
+}
+
+// one wave for each entry of the table (a bucket is a rectangle of distances), one more for each head's lam
+__global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a) {
+  const int h = blockIdx.y, b = blockIdx.x, lane = threadIdx.x;
+  double acc = 0.0;
+  if (b < a.ny * a.nx) {
+    if (!a.line) return;
+    int y0, y1, x0, x1;
+    bucket_range(b / a.nx, a.ny, a.gh, a.thr_y, y0, y1);
+    bucket_range(b % a.nx, a.nx, a.gw, a.thr_x, x0, x1);
+    const int w = max(x1 - x0, 0), n = max(y1 - y0, 0) * w;
+    const double* p = a.line + (int64_t)h * (2 * a.gh - 1) * (2 * a.gw - 1);
+    for (int e = lane; e < n; e += 64) acc += p[(int64_t)(y0 + e / w + a.gh - 1) * (2 * a.gw - 1) + x0 + e % w + a.gw - 1];
+  } else {
+    for (int s = lane; s < a.slots; s += 64) acc += (double)a.dlam_part[(int64_t)s * a.H + h];
+  }
+#pragma unroll
+  for (int s = 32; s >= 1; s >>= 1) acc += __shfl_xor(acc, s);
+  if (lane == 0) {
+    if (b < a.ny * a.nx) a.dtable[(int64_t)b * a.H + h] = (float)acc;
+    else a.dlam[h] = (float)acc;
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+static int ring_floats(const im2im_attention_desc* p) {
+  int n = 64;
+  while (n < window_floats(p->gh, p->gw)) n *= 2;
+  return n;
+}
+
+// images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, so their number (about 1024)
+// bounds that memory
+static void set_groups(AttnArgs* a) {
+  a->group_images = (int)std::max<int64_t>(1, std::min<int64_t>(a->B, (int64_t)a->B * a->H * a->nq / 1024));
+  a->groups = (int)cdiv(a->B, a->group_images);
+}
+
+struct BwdLayout { int64_t delta, part, line, dlam, bytes; };
+static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
+  const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  BwdLayout l;
+  l.delta = 0;
+  l.line = up((int64_t)a.B * a.H * maps * a.Lq * 4);
+  l.part = l.line + (table ? up((int64_t)a.H * a.line_len * 8) : 0);
+  l.dlam = l.part + (table ? up((int64_t)a.groups * a.nq * a.H * a.line_len * 4) : 0);
+  l.bytes = l.dlam + up((int64_t)a.groups * a.nq * a.H * 4);
+  return l;
+}
+
+template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, int window, hipStream_t st) {
+  auto kern = attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS>;
+  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 256 +
+                      (size_t)(BIAS ? 2 * WAVES * a.ring : 0) * 4 + (size_t)round64(window) * 4;
+  if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq)), dim3(64 * WAVES), smem, st, a);
+  return check_launch("attn_bwd_q_kernel");
+}
+
+template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, int window, float* delta, hipStream_t st) {
+  hipLaunchKernelGGL((attn_delta_kernel<T, MAPS>), dim3((unsigned)cdiv((int64_t)a.B * a.H * a.Lq, 16)), dim3(256), 0, st, a, delta);
+  if (int rc = check_launch("attn_delta_kernel")) return rc;
+  if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, window, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, window, st)) return rc;
+  auto kern = attn_bwd_kv_kernel<T, DQ, DV, MAPS>;
+  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 2 * MAPS * KEYS * 4 + (size_t)round64(window) * 4;
+  if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
+  return check_launch("attn_bwd_kv_kernel");
+}
+
+template <typename T> static int dispatch_bwd(const AttnArgs& a, int maps, int window, float* delta, hipStream_t st) {
+  if (maps == 2) return a.d <= 32 ? launch_bwd<T, 32, 64, 2>(a, window, delta, st) : launch_bwd<T, 64, 128, 2>(a, window, delta, st);
+  if (a.d <= 32) return launch_bwd<T, 32, 32, 1>(a, window, delta, st);
+  if (a.d <= 64) return launch_bwd<T, 64, 64, 1>(a, window, delta, st);
+  return launch_bwd<T, 128, 128, 1>(a, window, delta, st);
+}
+
+}  // namespace im2im
+
+using namespace im2im;
+
+extern "C" int64_t im2im_attention_bwd_workspace_bytes(const im2im_attention_desc* p, int32_t want_table) {
+  AttnArgs a = {};
+  if (attn_check(p, &a)) return -1;
+  set_groups(&a);
+  return bwd_layout(a, p->maps, want_table != 0).bytes;
+}
+
+extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_attention_grads* g, void* ws, int64_t ws_bytes,
+                                   im2im_stream_t stream) {
+  AttnArgs a = {};
+  if (int rc = attn_check(p, &a)) return rc;
+  IM2IM_REQUIRE(g != nullptr);
+  IM2IM_REQUIRE(g->dout && g->lse && g->map_out && g->dq && g->dk && g->dv);
+  IM2IM_REQUIRE(p->maps == 1 || g->dlam);
+  IM2IM_REQUIRE((reinterpret_cast<uintptr_t>(g->dout) & 15) == 0);
+  const int64_t e = p->dtype == IM2IM_BF16 ? 2 : 4;
+  const void* ptr[3] = {g->dq, g->dk, g->dv};
+  const int64_t* stride[3] = {g->dq_stride, g->dk_stride, g->dv_stride};
+  for (int t = 0; t < 3; ++t) {
+    IM2IM_REQUIRE((reinterpret_cast<uintptr_t>(ptr[t]) & 15) == 0);
+    for (int x = 0; x < 3; ++x) IM2IM_REQUIRE(stride[t][x] > 0 && (stride[t][x] * e) % 16 == 0);
+  }
+  const bool table = g->dtable != nullptr;
+  IM2IM_REQUIRE(!table || (g->ny >= 1 && g->ny <= 64 && (g->ny == 1 || g->ny % 2 == 0) && g->nx >= 1 && g->nx <= 64 && (g->nx == 1 || g->nx % 2 == 0)));
+  IM2IM_REQUIRE(!table || ((g->ny <= 2 || g->thr_y) && (g->nx <= 2 || g->thr_x)));
+  set_groups(&a);
+  const BwdLayout l = bwd_layout(a, p->maps, table);
+  IM2IM_REQUIRE(ws && ws_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
+  char* w = static_cast<char*>(ws);
+  float* delta = reinterpret_cast<float*>(w + l.delta);
+  a.dout = g->dout; a.lse = const_cast<float*>(g->lse); a.osave = const_cast<float*>(g->map_out); a.delta = delta;
+  a.dq = g->dq; a.dk = g->dk; a.dvv = g->dv;
+  for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
+  a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
+  a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
+  a.ring = ring_floats(p);
+  const int window = window_floats(p->gh, p->gw);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, window, delta, st) : dispatch_bwd<float>(a, p->maps, window, delta, st)) return rc;
+  double* line = reinterpret_cast<double*>(w + l.line);
+  if (table) {
+    hipLaunchKernelGGL(attn_line_sum_kernel, dim3((unsigned)cdiv(a.line_len, 64), (unsigned)a.H), dim3(256), 0, st, a, line);
+    if (int rc = check_launch("attn_line_sum_kernel")) return rc;
+  }
+  if (!table && p->maps == 1) return IM2IM_OK;
+  BucketArgs s = {};
+  s.line = table ? line : nullptr;
+  s.dlam_part = a.dlam_part; s.dtable = g->dtable; s.dlam = g->dlam;
+  s.ny = table ? g->ny : 0; s.nx = table ? g->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.nq;
+  for (int m = 0; m + 1 < s.ny / 2; ++m) s.thr_y[m] = g->thr_y[m];
+  for (int m = 0; m + 1 < s.nx / 2; ++m) s.thr_x[m] = g->thr_x[m];
+  hipLaunchKernelGGL(attn_bucket_sum_kernel, dim3((unsigned)(s.ny * s.nx + (p->maps == 2)), (unsigned)a.H), dim3(64), 0, st, s);
+  return check_launch("attn_bucket_sum_kernel");
+}

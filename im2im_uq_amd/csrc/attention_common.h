@@ -1,0 +1,158 @@
+// Shared pieces of the grid-attention kernels (attention_fwd.hip, attention_bwd.hip).
+//
+// Tokens are the pixels of a gh x gw grid in raster order.  With code(t) = (t / gw) * (2 gw - 1) + t % gw the learned bias of a
+// (query i, key j) pair is line[code(j) - code(i) + off], off = code(gh gw - 1): one vector per head, expanded from the bucket table
+// (im2im_relpos_line), so a pair's bias is one subtraction and one LDS read, and its gradient one LDS add.
+//
+// MFMA shape: v_mfma_f32_32x32x16_bf16 (fp32: four v_mfma_f32_32x32x2_f32 per 16-byte fragment).  In the 32 x 32 result lane l holds column
+// l % 32 and rows row(r) = 8 (r / 4) + 4 (l / 32) + r % 4, r = 0..15.  Scores are computed TRANSPOSED (keys as rows, queries as
+// columns; the key gradients the other way round): a softmax row then lives in one lane pair, its running maximum and sum are plain
+// per-lane registers, and the probabilities are already in the layout of the next product's right operand -- they never go through
+// LDS.  That product needs its left operand transposed: ds_read_b64_tr_b16 (fp32: scalar reads).
+#pragma once
+#include "common.h"
+#include "dtypes.h"
+
+namespace im2im {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  int64_t qs[3], ks[3], vs[3];        // element strides: batch, token, head
+  const float* line;                  // [H][line_len], in units of log2
+  const int32_t* lengths;             // [B] or null
+  const float* lam;                   // [H] (two maps)
+  int B, Lq, Lk, H, d, dv, gw, line_len, line_off, q_start, nq, nk;
+  float scale;                        // of the scores
+  // forward
+  void* out;                          // [B][Lq][H][dv]
+  float* lse;                         // [B*H][MAPS][Lq] (log2 units) or null
+  float* osave;                       // [B*H][Lq][MAPS][dv] or null: each map's own result in 32 bits
+  float* part;                        // split keys: [splits][B*H*Lq][MAPS][dv]
+  float* part_ml;                     //             [splits][B*H*Lq][MAPS][2]
+  int splits, tiles_per_split;
+  // backward
+  const void* dout;                   // [B][Lq][H][dv]
+  const float* delta;                 // [B*H][MAPS][Lq]
+  void *dq, *dk, *dvv;
+  int64_t dqs[3], dks[3], dvs[3];
+  float* line_part;                   // [nq * groups][H][line_len] or null
+  float* dlam_part;                   // [nq * groups][H]
+  int groups, group_images, ring;     // ring: floats in one copy of the LDS accumulator (a power of two)
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int KEYS = 64;              // keys (queries in the key-gradient kernel) of one LDS tile
+constexpr int WAVES = 4, ROWS = 32 * WAVES;   // queries (keys) of a workgroup: 32 columns for each wave
+
+template <typename T> struct Mma;
+template <> struct Mma<bf16_t> {
+  static constexpr int KC = 16, NE = 8;          // reduction length of a fragment, elements of it in a lane
+  using Frag = short8;
+  static __device__ __forceinline__ Frag zero() { return short8{0, 0, 0, 0, 0, 0, 0, 0}; }
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+  }
+  // result registers NE t .. NE t + NE - 1 as a right operand (the reduction order matches load_t's)
+  static __device__ __forceinline__ Frag pack(const f32x16& s, int t) {
+    bf16x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (__bf16)s[8 * t + e];
+    return __builtin_bit_cast(short8, r);
+  }
+  static __device__ __forceinline__ Frag pack_rest(const f32x16& s, Frag hi, int t) {   // what pack() rounded away
+    const bf16x8 h = as_bf16x8(hi);
+    bf16x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (__bf16)(s[8 * t + e] - (float)h[e]);
+    return __builtin_bit_cast(short8, r);
+  }
+  // left operand taken transposed from an LDS tile [rows][stride]: lane = column col0 + l % 32, reduction = rows row0 + row(NE t + e)
+  static __device__ __forceinline__ Frag load_t(const bf16_t* tile, int stride, int row0, int t, int col0) {
+    const int lane = threadIdx.x & 63, q = lane & 15;
+    const bf16_t* p = tile + (size_t)(row0 + 16 * t + 4 * (lane >> 5) + (q >> 2)) * stride + col0 + 16 * ((lane >> 4) & 1) + 4 * (q & 3);
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)reinterpret_cast<const char*>(p));
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)reinterpret_cast<const char*>(p + 8 * stride));
+    return short8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+};
+template <> struct Mma<float> {
+  static constexpr int KC = 8, NE = 4;
+  using Frag = f32x4;
+  static __device__ __forceinline__ Frag zero() { return f32x4{0.f, 0.f, 0.f, 0.f}; }
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ Frag pack(const f32x16& s, int t) { return f32x4{s[4 * t], s[4 * t + 1], s[4 * t + 2], s[4 * t + 3]}; }
+  static __device__ __forceinline__ Frag pack_rest(const f32x16&, Frag, int) { return zero(); }
+  static __device__ __forceinline__ Frag load_t(const float* tile, int stride, int row0, int t, int col0) {
+    const int lane = threadIdx.x & 63;
+    const float* p = tile + (size_t)(row0 + 8 * t + 4 * (lane >> 5)) * stride + col0 + (lane & 31);
+    return f32x4{p[0], p[stride], p[2 * stride], p[3 * stride]};
+  }
+};
+
+template <typename T> __device__ __forceinline__ typename Mma<T>::Frag load_frag(const T* p) { return *reinterpret_cast<const typename Mma<T>::Frag*>(p); }
+template <typename T> __host__ __device__ constexpr int padded(int d) { return d + 16 / (int)sizeof(T); }   // LDS row length: 16 rows' 16-byte reads on distinct banks
+
+__device__ __forceinline__ f32x16 zero16() { return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ int mfma_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+__device__ __forceinline__ int grid_code(int t, int gw) { return (t / gw) * (2 * gw - 1) + t % gw; }
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// a lane's right-operand fragments of one row (queries: columns of the transposed scores), zero behind the row's d elements
+template <typename T, int D> __device__ __forceinline__ void load_row_frags(typename Mma<T>::Frag* f, const T* row, bool valid, int d, int half) {
+#pragma unroll
+  for (int c = 0; c < D / Mma<T>::KC; ++c) {
+    const int at = c * Mma<T>::KC + half * Mma<T>::NE;
+    f[c] = valid && at < d ? load_frag<T>(row + at) : Mma<T>::zero();
+  }
+}
+
+// rows [0, NR) of a tile into LDS by the whole workgroup; rows from `valid` on and elements from d on are zeros (masked rows may hold
+// anything, infinities and NaN too: a zero probability does not silence them in a product, a zero operand does)
+template <typename T, int D, int NR> __device__ __forceinline__ void stage_rows(T* dst, const T* src, int64_t stride, int valid, int d) {
+  constexpr int V = 16 / (int)sizeof(T), PR = D / V, S = padded<T>(D);
+#pragma unroll
+  for (int i0 = 0; i0 < NR * PR; i0 += 64 * WAVES) {
+    const int i = i0 + threadIdx.x;
+    if (NR * PR % (64 * WAVES) == 0 || i < NR * PR) {
+      const int r = i / PR, c = (i % PR) * V;
+      u32x4 x = {0, 0, 0, 0};
+      if (r < valid && c < d) x = *reinterpret_cast<const u32x4*>(src + r * stride + c);
+      *reinterpret_cast<u32x4*>(dst + r * S + c) = x;
+    }
+  }
+}
+
+// four consecutive elements (16 bytes of fp32, 8 bytes of bf16)
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
+__device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<bf16x4*>(p) = bf16x4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+}
+
+// a contiguous band of the work list for each of the 8 XCDs (workgroups are dealt to them round-robin), so that the workgroups that share
+// an image and head share an L2
+__device__ __forceinline__ int xcd_band(int id, int total) {
+  const int each = total >> 3, more = total & 7, x = id & 7;
+  return x * each + (x < more ? x : more) + (id >> 3);
+}
+
+// window of `line` that n consecutive tokens x KEYS tokens can reach, in floats
+inline int code_span(int64_t n, int gh, int gw) {
+  if (gh == 1) return (int)n - 1;
+  int64_t rows = (n - 1 + gw - 1) / gw;
+  if (rows > gh - 1) rows = gh - 1;
+  return (int)(n - 1 + rows * (gw - 1));
+}
+inline int window_floats(int gh, int gw) { return code_span(ROWS, gh, gw) + code_span(KEYS, gh, gw) + 1; }
+inline int round64(int n) { return (n + 63) / 64 * 64; }
+
+int attn_check(const im2im_attention_desc* p, AttnArgs* a);      // validates the description, fills the common fields
+int attn_allow_lds(const void* kernel, size_t bytes);            // raises the kernel's dynamic LDS limit on the current device
+
+}  // namespace im2im

@@ -1,0 +1,394 @@
+// Grid attention, forward: softmax attention over the pixels of a grid with a learned relative position bias, and its
+// differential form (the difference of two softmax maps that share the values).
+//   s_ij = scale q_i . k_j + bias(j - i),   o_i = sum_j softmax_j(s_i)_j v_j          (keys from lengths[b] on take no part)
+//   two maps: o = o1 - lam o2
+// One pass over the keys with a running maximum and sum; work split over the keys and joined when there are few queries.
+#include "attention_common.h"
+#include <cmath>
+#include <mutex>
+#include <unordered_map>
+
+namespace im2im {
+
+// ---------------------------------------------------------------------------------------------------------- bias table -> line
+struct LineArgs {
+  const float* table;    // [ny][nx][H]
+  float* line;           // [H][line_len]
+  int ny, nx, H, gh, gw, len;
+  int thr_y[32], thr_x[32];   // smallest distance of bucket 1, 2, ...
+};
+
+__device__ __forceinline__ int axis_bucket(int delta, int n, const int* thr) {
+  if (n == 1) return 0;
+  const int side = n / 2, t = delta < 0 ? -delta : delta;
+  int b = 0;
+  for (int m = 0; m < side - 1; ++m) b += t >= thr[m];
+  return b + (delta > 0 ? side : 0);
+}
+
+// a few thousand floats: bound by its launch
+__global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
+  const int idx = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+  if (idx >= a.len) return;
+  const int w = 2 * a.gw - 1;
+  const int b = axis_bucket(idx / w - (a.gh - 1), a.ny, a.thr_y) * a.nx + axis_bucket(idx % w - (a.gw - 1), a.nx, a.thr_x);
+  const float t = a.table[(int64_t)b * a.H + h];
+  // a finite entry stays finite in units of log2 (the type's lowest value is a large bias; -infinity is a mask)
+  float v = t * LOG2E;
+  if (v == -INFINITY && t != -INFINITY) v = -1.7e38f;
+  a.line[(int64_t)h * a.len + idx] = v;
+}
+
+// ------------------------------------------------------------------------------------------------------------------- forward
+// One workgroup: 128 queries (a wave has 32 of them as its columns), keys in tiles of 64 through LDS.
+// SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
+// result exact to about 2^-18: the backward's row sums D = dO . O are taken from it, and the table's gradient, a 32-bit sum with much
+// cancellation, would carry a rounding of P to bf16 (2^-9) in every D.
+template <typename T, int DQ, int DV, int MAPS, bool SAVE>
+__global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NB = DV / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  T* Ks = reinterpret_cast<T*>(smem);
+  T* Vs = Ks + MAPS * KEYS * SQ;
+  int* kc = reinterpret_cast<int*>(Vs + KEYS * SV);
+  float* win = reinterpret_cast<float*>(kc + KEYS);
+
+  const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.splits, item = lin / a.splits;
+  const int qt = item % a.nq, bh = item / a.nq, h = bh % a.H, b = bh / a.H;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int i0 = qt * ROWS, i_last = min(i0 + ROWS, a.Lq) - 1;
+  const int i = i0 + wave * 32 + (lane & 31);
+  const bool mine = i < a.Lq, busy = i0 + wave * 32 < a.Lq;
+  const int code_last = grid_code(a.q_start + i_last, a.gw);
+  const int aoff = code_last - grid_code(a.q_start + min(i, i_last), a.gw);
+  const int qspan = code_last - grid_code(a.q_start + i0, a.gw);
+  const float scale2 = a.scale * LOG2E;
+
+  Frag qf[MAPS][DQ / M::KC];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m)
+    load_row_frags<T, DQ>(qf[m], static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)min(i, i_last) * a.qs[1] + (int64_t)(MAPS * h + m) * a.qs[2],
+                          mine, a.d, half);
+  float mx[MAPS], sum[MAPS];
+  f32x16 o[MAPS][NB];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    mx[m] = -INFINITY;
+    sum[m] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) o[m][n] = zero16();
+  }
+
+  const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
+  const int t0 = sp * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, (len + KEYS - 1) / KEYS);
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)(MAPS * h) * a.ks[2];
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
+  const float* line = a.line + (int64_t)h * a.line_len;
+
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = t * KEYS, valid = min(len - j0, KEYS);
+    const int kfirst = grid_code(j0, a.gw), base = kfirst - code_last + a.line_off;
+    const int wlen = grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Ks + m * KEYS * SQ, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
+    stage_rows<T, DV, KEYS>(Vs, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+    if (threadIdx.x < KEYS) kc[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
+    for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
+    __syncthreads();
+    if (!busy) continue;
+
+    f32x16 s[MAPS][2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      float bias[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) bias[r] = win[kc[sub * 32 + mfma_row(r, half)] + aoff];
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        f32x16 acc = zero16();
+#pragma unroll
+        for (int c = 0; c < DQ / M::KC; ++c)
+          acc = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], acc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[m][sub][r] = fmaf(acc[r], scale2, bias[r]);
+      }
+    }
+    if (valid < KEYS) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (sub * 32 + mfma_row(r, half) >= valid)
+#pragma unroll
+            for (int m = 0; m < MAPS; ++m) s[m][sub][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      float top = s[m][0][0];
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[m][sub][r]);
+      top = fmaxf(mx[m], fmaxf(top, __shfl_xor(top, 32)));
+      const float ref = top == -INFINITY ? 0.f : top;          // nothing but masks so far
+      const float shrink = exp2_(mx[m] - ref);
+      mx[m] = top;
+      float add = 0.f;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[m][sub][r] = exp2_(s[m][sub][r] - ref);
+          add += s[m][sub][r];
+        }
+      sum[m] = sum[m] * shrink + add;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][n][r] *= shrink;
+    }
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int ks = 0; ks < 32 / M::KC; ++ks) {
+        Frag pf[MAPS], pr[MAPS];
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) {
+          pf[m] = M::pack(s[m][sub], ks);
+          if (SAVE && sizeof(T) == 2) pr[m] = M::pack_rest(s[m][sub], pf[m], ks);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const Frag vf = M::load_t(Vs, SV, sub * 32, ks, n * 32);
+#pragma unroll
+          for (int m = 0; m < MAPS; ++m) {
+            o[m][n] = M::mma(vf, pf[m], o[m][n]);
+            if (SAVE && sizeof(T) == 2) o[m][n] = M::mma(vf, pr[m], o[m][n]);
+          }
+        }
+      }
+  }
+
+  if (!busy) return;
+  const int64_t row = (int64_t)bh * a.Lq + i;
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) sum[m] += __shfl_xor(sum[m], 32);
+  if (!mine) return;
+  if (a.splits > 1) {                                             // joined by attn_combine_kernel
+    const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      const int64_t at = ((int64_t)sp * rows + row) * MAPS + m;
+      if (half == 0) {
+        a.part_ml[at * 2] = mx[m];
+        a.part_ml[at * 2 + 1] = sum[m];
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = n * 32 + 8 * g + 4 * half;
+          if (c < a.dv) store4(a.part + at * a.dv + c, o[m][n][4 * g], o[m][n][4 * g + 1], o[m][n][4 * g + 2], o[m][n][4 * g + 3]);
+        }
+    }
+    return;
+  }
+  float inv[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    inv[m] = sum[m] > 0.f ? 1.f / sum[m] : 0.f;                   // no key at all: a row of zeros
+    if (SAVE && half == 0)                                        // +infinity there: the backward's probabilities come out as zeros
+      a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum[m] > 0.f ? mx[m] + __builtin_amdgcn_logf(sum[m]) : INFINITY;
+  }
+  const float lam = MAPS == 2 ? a.lam[h] : 0.f;
+  T* out = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = n * 32 + 8 * g + 4 * half;
+      if (c >= a.dv) continue;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = o[0][n][4 * g + e] * inv[0];
+        if (MAPS == 2) v[e] -= lam * (o[MAPS - 1][n][4 * g + e] * inv[MAPS - 1]);
+      }
+      store4(out + c, v[0], v[1], v[2], v[3]);
+      if (SAVE)
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m)
+          store4(a.osave + (row * MAPS + m) * a.dv + c, o[m][n][4 * g] * inv[m], o[m][n][4 * g + 1] * inv[m], o[m][n][4 * g + 2] * inv[m],
+                 o[m][n][4 * g + 3] * inv[m]);
+    }
+}
+
+// joins the parts of a row: 32 lanes for each row, four channels a lane
+template <typename T, int MAPS> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs a) {
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int c = (threadIdx.x & 31) * 4, i = (int)(row % a.Lq), bh = (int)(row / a.Lq), h = bh % a.H, b = bh / a.H;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[((s * rows + row) * MAPS + m) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      const int64_t at = (s * rows + row) * MAPS + m;
+      const float w = exp2_(a.part_ml[at * 2] - ref);
+      sum += w * a.part_ml[at * 2 + 1];
+      if (c < a.dv) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * a.dv + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += w * x[e];
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    if (a.lse && c == 0) a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum > 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] *= inv;
+      v[e] += m == 0 ? o[e] : -a.lam[h] * o[e];
+    }
+    if (a.osave && c < a.dv) store4(a.osave + (row * MAPS + m) * a.dv + c, o[0], o[1], o[2], o[3]);
+  }
+  if (c < a.dv) store4(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv + c, v[0], v[1], v[2], v[3]);
+}
+
+// -------------------------------------------------------------------------------------------------------------------- host
+int attn_allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return IM2IM_OK;
+  static std::mutex mu;
+  static std::unordered_map<const void*, size_t> set[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return fail_invalid("attention: device index");
+  std::lock_guard<std::mutex> lock(mu);
+  size_t& have = set[dev][kernel];
+  if (bytes > have) {
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != hipSuccess) {
+      (void)hipGetLastError();
+      return fail_invalid("attention: the device refuses the kernel's LDS size");
+    }
+    have = bytes;
+  }
+  return IM2IM_OK;
+}
+
+int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
+  IM2IM_REQUIRE(p != nullptr);
+  IM2IM_REQUIRE(p->q && p->k && p->v && p->line);
+  IM2IM_REQUIRE(p->dtype == IM2IM_F32 || p->dtype == IM2IM_BF16);
+  IM2IM_REQUIRE(p->maps == 1 || p->maps == 2);
+  IM2IM_REQUIRE(p->maps == 1 || p->lam != nullptr);
+  IM2IM_REQUIRE(p->B >= 1 && p->Lq >= 1 && p->Lk >= 1 && p->H >= 1);
+  IM2IM_REQUIRE(p->D >= 8 && p->D % 8 == 0 && p->D * p->maps <= 128);
+  IM2IM_REQUIRE(p->gh >= 1 && p->gw >= 1 && (p->gh == 1 || p->gw <= 512));
+  IM2IM_REQUIRE((int64_t)p->gh * p->gw <= (1 << 24));
+  IM2IM_REQUIRE(p->Lk <= p->gh * p->gw);
+  IM2IM_REQUIRE(p->q_start >= 0 && p->q_start <= p->gh * p->gw - p->Lq);
+  IM2IM_REQUIRE(std::isfinite(p->scale));
+  const int64_t e = p->dtype == IM2IM_BF16 ? 2 : 4;
+  const void* ptr[3] = {p->q, p->k, p->v};
+  const int64_t* st[3] = {p->q_stride, p->k_stride, p->v_stride};
+  for (int t = 0; t < 3; ++t) {
+    IM2IM_REQUIRE((reinterpret_cast<uintptr_t>(ptr[t]) & 15) == 0);
+    for (int x = 0; x < 3; ++x) IM2IM_REQUIRE(st[t][x] >= 0 && (st[t][x] * e) % 16 == 0);
+  }
+  a->q = p->q; a->k = p->k; a->v = p->v;
+  for (int x = 0; x < 3; ++x) { a->qs[x] = p->q_stride[x]; a->ks[x] = p->k_stride[x]; a->vs[x] = p->v_stride[x]; }
+  a->line = p->line; a->lengths = p->lengths; a->lam = p->lam;
+  a->B = p->B; a->Lq = p->Lq; a->Lk = p->Lk; a->H = p->H; a->d = p->D; a->dv = p->D * p->maps; a->gw = p->gw;
+  a->line_len = (2 * p->gh - 1) * (2 * p->gw - 1);
+  a->line_off = (p->gh - 1) * (2 * p->gw - 1) + p->gw - 1;
+  a->q_start = p->q_start;
+  a->nq = (int)cdiv(p->Lq, ROWS);
+  a->nk = (int)cdiv(p->Lk, ROWS);
+  a->scale = p->scale;
+  IM2IM_REQUIRE((int64_t)p->B * p->H * p->Lq < (1ll << 31) && (int64_t)p->B * p->H * a->nk < (1ll << 31) / 64);
+  return IM2IM_OK;
+}
+
+// Parts of the keys: with fewer workgroups than two for each of the 256 CUs the rest of the chip takes key tiles (a single token against
+// 4096 keys: 8 workgroups without).
+static int key_splits(const AttnArgs& a) {
+  const int64_t items = (int64_t)a.B * a.H * a.nq, tiles = cdiv(a.Lk, KEYS);
+  if (items >= 256 || tiles < 2) return 1;
+  int64_t n = cdiv(512, items);
+  if (n > tiles) n = tiles;
+  return (int)cdiv(tiles, cdiv(tiles, n));
+}
+
+template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, int window, hipStream_t st) {
+  auto kern = attn_fwd_kernel<T, DQ, DV, MAPS, SAVE>;
+  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + (size_t)round64(window) * 4;
+  if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nq * a.splits)), dim3(64 * WAVES), smem, st, a);
+  if (int rc = check_launch("attn_fwd_kernel")) return rc;
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((attn_combine_kernel<T, MAPS>), dim3((unsigned)cdiv((int64_t)a.B * a.H * a.Lq, 8)), dim3(256), 0, st, a);
+    return check_launch("attn_combine_kernel");
+  }
+  return IM2IM_OK;
+}
+
+template <typename T, bool SAVE> static int dispatch_fwd(const AttnArgs& a, int maps, int window, hipStream_t st) {
+  if (maps == 2) return a.d <= 32 ? launch_fwd<T, 32, 64, 2, SAVE>(a, window, st) : launch_fwd<T, 64, 128, 2, SAVE>(a, window, st);
+  if (a.d <= 32) return launch_fwd<T, 32, 32, 1, SAVE>(a, window, st);
+  if (a.d <= 64) return launch_fwd<T, 64, 64, 1, SAVE>(a, window, st);
+  return launch_fwd<T, 128, 128, 1, SAVE>(a, window, st);
+}
+
+}  // namespace im2im
+
+using namespace im2im;
+
+extern "C" int64_t im2im_relpos_line_len(int32_t gh, int32_t gw) {
+  if (gh < 1 || gw < 1 || (int64_t)gh * gw > (1 << 24)) return -1;
+  return (int64_t)(2 * gh - 1) * (2 * gw - 1);
+}
+
+extern "C" int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, const int32_t* thr_y, const int32_t* thr_x, int32_t gh,
+                                 int32_t gw, float* line, im2im_stream_t stream) {
+  IM2IM_REQUIRE(table && line && H >= 1 && H <= 65535);
+  IM2IM_REQUIRE(ny >= 1 && ny <= 64 && (ny == 1 || ny % 2 == 0) && nx >= 1 && nx <= 64 && (nx == 1 || nx % 2 == 0));
+  IM2IM_REQUIRE(gh >= 1 && gw >= 1 && (int64_t)gh * gw <= (1 << 24));
+  IM2IM_REQUIRE((ny <= 2 || thr_y) && (nx <= 2 || thr_x));
+  LineArgs a = {};
+  a.table = table; a.line = line; a.ny = ny; a.nx = nx; a.H = H; a.gh = gh; a.gw = gw; a.len = (2 * gh - 1) * (2 * gw - 1);
+  for (int m = 0; m + 1 < ny / 2; ++m) a.thr_y[m] = thr_y[m];
+  for (int m = 0; m + 1 < nx / 2; ++m) a.thr_x[m] = thr_x[m];
+  hipLaunchKernelGGL(relpos_line_kernel, dim3((unsigned)cdiv(a.len, 256), (unsigned)H), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  return check_launch("relpos_line_kernel");
+}
+
+extern "C" int64_t im2im_attention_fwd_workspace_bytes(const im2im_attention_desc* p) {
+  AttnArgs a = {};
+  if (attn_check(p, &a)) return -1;
+  const int n = key_splits(a);
+  return n < 2 ? 0 : (int64_t)n * a.B * a.H * a.Lq * p->maps * (a.dv + 2) * 4;
+}
+
+extern "C" int im2im_attention_fwd(const im2im_attention_desc* p, void* out, float* lse, float* map_out, void* ws, int64_t ws_bytes,
+                                   im2im_stream_t stream) {
+  AttnArgs a = {};
+  if (int rc = attn_check(p, &a)) return rc;
+  IM2IM_REQUIRE(out && (lse != nullptr) == (map_out != nullptr));
+  a.out = out; a.lse = lse; a.osave = map_out;
+  a.splits = key_splits(a);
+  a.tiles_per_split = (int)cdiv(cdiv(a.Lk, KEYS), a.splits);
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.splits * a.B * a.H * a.Lq * p->maps;
+    IM2IM_REQUIRE(ws && ws_bytes >= rows * (a.dv + 2) * 4);
+    a.part = static_cast<float*>(ws);
+    a.part_ml = a.part + rows * a.dv;
+  }
+  const int window = window_floats(p->gh, p->gw);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p->dtype == IM2IM_BF16) return lse ? dispatch_fwd<bf16_t, true>(a, p->maps, window, st) : dispatch_fwd<bf16_t, false>(a, p->maps, window, st);
+  return lse ? dispatch_fwd<float, true>(a, p->maps, window, st) : dispatch_fwd<float, false>(a, p->maps, window, st);
+}

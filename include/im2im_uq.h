@@ -563,6 +563,74 @@ int im2im_fastmri_abs_normalize(const float* in, float* out, int32_t B, int32_t 
 int im2im_center_crop_affine(const float* in, float* out, int64_t B, int32_t Hin, int32_t Win, int32_t H,
                              int32_t W, float sub, float div, im2im_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Attention bottleneck (build-side operators; the reference's trunk has none).  Tokens are the pixels of a gh x gw grid in raster order.
+ *
+ * Relative position bias by buckets: bias(query, key) = table[by(y_key - y_query)][bx(x_key - x_query)][h].  An axis with n buckets (1 or an even
+ * number, at most 64) gives n / 2 to the distances <= 0 and n / 2 to those > 0 (n = 1: everything in one); of these n / 2, bucket m holds the
+ * distances |d| >= thr[m - 1] (and < thr[m]): thr is a HOST array of n / 2 - 1 ascending numbers (null where that is 0).
+ *   im2im_relpos_line: table [ny][nx][H] fp32 -> line [H][im2im_relpos_line_len(gh, gw)] fp32, the bias of every displacement times log2(e):
+ *     what the attention entry points read. */
+int64_t im2im_relpos_line_len(int32_t gh, int32_t gw);
+int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, const int32_t* thr_y, const int32_t* thr_x, int32_t gh,
+                      int32_t gw, float* line, im2im_stream_t stream);
+
+/* Softmax attention over the grid (maps = 1) and its differential form (maps = 2):
+ *   s = scale q . k + bias,  P = softmax over the keys j < lengths[b],  out = P v;   maps = 2: out = (P_0 - lam[h] P_1) v.
+ *   q [B][Lq][H*maps][D], k [B][Lk][H*maps][D], v [B][Lk][H][D*maps]; map m of head h is head h*maps + m of q and k.  The last index is dense,
+ *   the strides of the others are elements {batch, token, head}; rows start at 16 bytes.  D a multiple of 8, D*maps <= 128.
+ *   The queries are the grid's tokens q_start .. q_start + Lq - 1, the keys its tokens 0 .. Lk - 1 (gw <= 512 unless gh == 1).
+ *   lengths: device int32 [B] or null (all Lk), clipped to 0..Lk; keys behind it take no part, whatever they hold; a row without
+ *   keys gives zeros (and zero gradients).  A table entry of -infinity masks its pairs.
+ *   lse / map_out (both or neither): saved for the backward: lse [B*H][maps][Lq] fp32, map_out [B*H][Lq][maps][D*maps] fp32.
+ * im2im_attention_bwd: dout [B][Lq][H][D*maps] dense; dq / dk / dv in the types and index order of q / k / v with their own strides; dtable
+ *   [ny][nx][H] fp32 or null; dlam [H] fp32 (maps = 2).  Every sum has a fixed order: repeated calls give the same bits. */
+typedef struct {
+  const void *q, *k, *v;
+  const float* line;
+  const int32_t* lengths;
+  const float* lam;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  int32_t B, Lq, Lk, H, D, maps, gh, gw, q_start, dtype;
+  float scale;
+} im2im_attention_desc;
+typedef struct {
+  const void* dout;
+  const float *lse, *map_out;
+  void *dq, *dk, *dv;
+  float *dtable, *dlam;
+  const int32_t *thr_y, *thr_x;
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+  int32_t ny, nx;
+} im2im_attention_grads;
+int64_t im2im_attention_fwd_workspace_bytes(const im2im_attention_desc* p);
+int im2im_attention_fwd(const im2im_attention_desc* p, void* out, float* lse, float* map_out, void* ws, int64_t ws_bytes,
+                        im2im_stream_t stream);
+int64_t im2im_attention_bwd_workspace_bytes(const im2im_attention_desc* p, int32_t want_table);
+int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_attention_grads* g, void* ws, int64_t ws_bytes,
+                        im2im_stream_t stream);
+
+/* The seam between two blocks: y = x + scale o sigmoid(gate) o N_post(f), h = N_pre(y) (from y in 32 bits), N over the C <= 8192 channels of a row:
+ *   IM2IM_NORM_RMS    v / sqrt(mean v^2 + eps) * weight
+ *   IM2IM_NORM_LAYER  (v - mean) / sqrt(var + eps) * weight + bias
+ * x, f, gate [rows][C] with row strides in elements (0: one row for all); f == null: h = N_pre(x) alone; gate, scale, the biases and pre_weight (no h)
+ * may be null.  Weights fp32 [C], starting at 16 bytes; y, h and all gradients of rows dense.  The backward takes dy and dh (one may be
+ * null: zero) and writes what is not null; sums over rows are 32-bit within a workgroup, 64-bit across, in a fixed order. */
+#define IM2IM_NORM_RMS 0
+#define IM2IM_NORM_LAYER 1
+typedef struct {
+  const void *x, *f, *gate;
+  const float *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+  int64_t rows, x_stride, f_stride, gate_stride;
+  int32_t C, norm, dtype;
+  float eps;
+} im2im_norm_gate_desc;
+int im2im_norm_gate_fwd(const im2im_norm_gate_desc* p, void* y, void* h, im2im_stream_t stream);
+int64_t im2im_norm_gate_bwd_workspace_bytes(int64_t rows, int32_t C);
+int im2im_norm_gate_bwd(const im2im_norm_gate_desc* p, const void* dy, const void* dh, void* dx, void* df, void* dgate, float* dscale,
+                        float* dpost_weight, float* dpost_bias, float* dpre_weight, float* dpre_bias, void* ws, int64_t ws_bytes,
+                        im2im_stream_t stream);
+
 /* Multi-tensor Adam: optim.Adam(net.parameters(), lr) at core/scripts/train.py:120 with torch
  * defaults (betas, eps, no weight decay, no amsgrad).  Host arrays of n_tensors device pointers / sizes;
  * `step` is the 1-based step count used for bias correction. */
