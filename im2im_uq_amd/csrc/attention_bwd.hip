@@ -33,15 +33,30 @@ template <typename T, int MAPS> __global__ __launch_bounds__(256) void attn_delt
   }
 }
 
+// a place of the ring, summed over its copies in their order, and zeros in its place
+template <bool ROW4> __device__ __forceinline__ double take_place(double* ring, unsigned place, unsigned size) {
+  double s = 0.0, *at = ring + place;
+#pragma unroll
+  for (int c = 0; c < 2 * WAVES; ++c, at += size + 4) {
+    s += at[0];
+    at[0] = 0.0;
+    if (ROW4 && place < 3) {                                      // what ran over the end
+      s += at[size];
+      at[size] = 0.0;
+    }
+  }
+  return s;
+}
+
 // -------------------------------------------------------------------------------------- queries' gradients, bias and lam
 // One workgroup: 128 queries of one head, of `group_images` images in turn, against their keys in tiles of 64.
 // Bias gradient: a pair's place in the line is code(j) - code(i) + off.  Within one instruction 32 lanes have 32 different queries and the
 // same key, so their places differ; the other 32 lanes have another key and add to a copy of their own; each wave has its own pair
 // of copies and its additions are in program order: no order is left open.  A copy is a ring over the line's index: the places
-// that the following tiles cannot reach any more are summed over the copies and written, each once (bias gradient = one LDS addition a
-// pair, and 2 gw + 128 floats a tile).
-template <typename T, int DQ, int DV, int MAPS, bool BIAS>
-__global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a) {
+// that the following tiles cannot reach any more are summed over the copies and written, each once.  The copies are 64-bit:
+// ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 3xx us at 78 images of 20 x 20, 8 x 64.
+template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4>
+__global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
@@ -50,8 +65,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
   T* Vs = Ks + MAPS * KEYS * SQ;
   int* kc = reinterpret_cast<int*>(Vs + KEYS * SV);
   float* red = reinterpret_cast<float*>(kc + KEYS);              // [WAVES]
-  float* ring = red + 64;                                        // [2 * WAVES][a.ring]
-  float* win = ring + (BIAS ? 2 * WAVES * a.ring : 0);
+  double* ring = reinterpret_cast<double*>(red + 64);            // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
+  float* win = reinterpret_cast<float*>(ring + (BIAS ? 2 * WAVES * (a.ring + 4) : 0));
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, gh_ = lin / a.nq, h = gh_ % a.H, group = gh_ / a.H;
   const int slot = group * a.nq + qt;
@@ -64,14 +79,14 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
   const int qspan = code_last - grid_code(a.q_start + i0, a.gw);
   const float scale2 = a.scale * LOG2E, lam = MAPS == 2 ? a.lam[h] : 0.f;
   const float* line = a.line + (int64_t)h * a.line_len;
-  const int mask = a.ring - 1;
-  float* my_ring = ring + (wave * 2 + half) * a.ring;
+  const unsigned size = a.ring, copy = size + 4;
+  double* my_ring = ring + (wave * 2 + half) * copy;
   float* line_out = BIAS ? a.line_part + ((int64_t)slot * a.H + h) * a.line_len : nullptr;
   const int line_begin = a.line_off - code_last, line_end = grid_code(a.Lk - 1, a.gw) - code_last + a.line_off + qspan + 1;
   float dlam = 0.f;
 
   if (BIAS)
-    for (int w = threadIdx.x; w < 2 * WAVES * a.ring; w += 64 * WAVES) ring[w] = 0.f;
+    for (int w = threadIdx.x; w < 2 * WAVES * (int)copy; w += 64 * WAVES) ring[w] = 0.0;
 
   const int b0 = group * a.group_images, b1 = min(b0 + a.group_images, a.B);
   for (int b = b0; b < b1; ++b) {
@@ -104,16 +119,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
       __syncthreads();
       if (BIAS) {                                                // a place's thread is the same for every image
         for (int w = done + ((int)threadIdx.x - done & 255); w < base; w += 64 * WAVES) {
-          float s = 0.f;
-#pragma unroll
-          for (int c = 0; c < 2 * WAVES; ++c) {
-            s += ring[c * a.ring + (w & mask)];
-            ring[c * a.ring + (w & mask)] = 0.f;
-          }
-          line_out[w] = b == b0 ? s : line_out[w] + s;
+          const double s = take_place<ROW4>(ring, (unsigned)w % size, size);
+          line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
         }
         done = base;
       }
+      const unsigned ring_base = (unsigned)base % size;
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Ks + m * KEYS * SQ, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
       stage_rows<T, DV, KEYS>(Vs, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
@@ -122,12 +133,13 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
       __syncthreads();
       if (!busy) continue;
 
-#pragma unroll
+#pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
-        f32x16 dp = zero16(), s[MAPS];
-#pragma unroll
-        for (int c = 0; c < DV / M::KC; ++c)
-          dp = M::mma(load_frag<T>(Vs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), gf[c], dp);
+        if (sub * 32 >= valid) break;
+        float bias[16];
+        window_bias<ROW4>(bias, win, kc + sub * 32, aoff, half);
+        // one map: the accumulators start at -D, the product ends at dP - D
+        f32x16 dp = splat16(MAPS == 1 ? -del[0] : 0.f), s[MAPS];
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
           s[m] = zero16();
@@ -136,20 +148,40 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
             s[m] = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], s[m]);
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int j = sub * 32 + mfma_row(r, half), w = kc[j] + aoff;
-          const float bias = win[w];
-          float ds[MAPS], total = 0.f;
+        for (int c = 0; c < DV / M::KC; ++c)
+          dp = M::mma(load_frag<T>(Vs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), gf[c], dp);
 #pragma unroll
-          for (int m = 0; m < MAPS; ++m) {
-            float p = exp2_(fmaf(s[m][r], scale2, bias) - lse[m]);
-            p = j < valid ? p : 0.f;
-            if (m == 1) dlam = fmaf(p, dp[r], dlam);
-            ds[m] = p * ((m == 0 ? dp[r] : -lam * dp[r]) - del[m]);
-            s[m][r] = ds[m];
-            total += ds[m];
+        for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[m][r] = exp2_(fmaf(s[m][r], scale2, bias[r]) - lse[m]);
+        if (valid < sub * 32 + 32) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (sub * 32 + mfma_row(r, half) >= valid)
+#pragma unroll
+              for (int m = 0; m < MAPS; ++m) s[m][r] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if constexpr (MAPS == 1) {
+            s[0][r] *= dp[r];
+            bias[r] = s[0][r];
+          } else {
+            dlam = fmaf(s[1][r], dp[r], dlam);
+            s[0][r] *= dp[r] - del[0];
+            s[1][r] *= fmaf(-lam, dp[r], -del[1]);
+            bias[r] = s[0][r] + s[1][r];
           }
-          if (BIAS) __hip_atomic_fetch_add(my_ring + (base + w & mask), total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        if (BIAS) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned at = ring_base + kc[sub * 32 + 8 * g + 4 * half + (ROW4 ? 0 : e)] + aoff;                  // < 2 size
+              __hip_atomic_fetch_add(my_ring + min(at, at - size) + (ROW4 ? e : 0), (double)bias[4 * g + e], __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
         }
 #pragma unroll
         for (int ks = 0; ks < 32 / M::KC; ++ks)
@@ -165,15 +197,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
     if (BIAS) {
       __syncthreads();
       for (int w = done + ((int)threadIdx.x - done & 255); w < line_end; w += 64 * WAVES) {
-        float s = 0.f;
-        if (w - done < a.ring) {
-#pragma unroll
-          for (int c = 0; c < 2 * WAVES; ++c) {
-            s += ring[c * a.ring + (w & mask)];
-            ring[c * a.ring + (w & mask)] = 0.f;
-          }
-        }
-        line_out[w] = b == b0 ? s : line_out[w] + s;
+        const double s = w - done < a.ring ? take_place<ROW4>(ring, (unsigned)w % size, size) : 0.0;
+        line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
       }
     }
     if (mine) {
@@ -203,8 +228,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(const AttnArgs a
 
 // ---------------------------------------------------------------------------------------------- keys' and values' gradients
 // One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.
-template <typename T, int DQ, int DV, int MAPS>
-__global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs a) {
+template <typename T, int DQ, int DV, int MAPS, bool ROW4>
+__global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
@@ -213,7 +238,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs 
   T* Gs = Qs + MAPS * KEYS * SQ;
   int* qc = reinterpret_cast<int*>(Gs + KEYS * SV);
   float* rows = reinterpret_cast<float*>(qc + KEYS);             // [2][MAPS][KEYS]: log-sums, D
-  float* win = rows + 2 * MAPS * KEYS;
+  float* win = rows + 2 * MAPS * KEYS + 4;                       // four zeros in front: behind the last query a run of four reaches there
+  if (threadIdx.x < 4) win[(int)threadIdx.x - 4] = 0.f;
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
@@ -251,7 +277,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs 
     stage_rows<T, DV, KEYS>(Gs, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, valid, a.dv);
     if (threadIdx.x < KEYS) {
       const int i = min((int)threadIdx.x, valid - 1);
-      qc[threadIdx.x] = code_last - grid_code(a.q_start + i0 + i, a.gw);
+      qc[threadIdx.x] = code_last - grid_code(a.q_start + i0 + i, a.gw);   // falls along the row
     }
     for (int w = threadIdx.x; w < MAPS * KEYS; w += 64 * WAVES) {
       const int m = w / KEYS, i = w % KEYS;
@@ -263,12 +289,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs 
     __syncthreads();
     if (!busy) continue;
 
-#pragma unroll
+#pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
+      if (sub * 32 >= valid) break;
+      float bias[16];
+      window_bias<ROW4, -1>(bias, win, qc + sub * 32, koff, half);
       f32x16 dp = zero16(), s[MAPS], mix;
-#pragma unroll
-      for (int c = 0; c < DV / M::KC; ++c)
-        dp = M::mma(load_frag<T>(Gs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), vf[c], dp);
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
         s[m] = zero16();
@@ -277,19 +303,22 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs 
           s[m] = M::mma(load_frag<T>(Qs + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), kf[m][c], s[m]);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = sub * 32 + mfma_row(r, half);
-        const float bias = win[qc[i] + koff];
-        float sum = 0.f;
+      for (int c = 0; c < DV / M::KC; ++c)
+        dp = M::mma(load_frag<T>(Gs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), vf[c], dp);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
-          float p = exp2_(fmaf(s[m][r], scale2, bias) - rows[m * KEYS + i]);
-          p = mine ? p : 0.f;
-          sum = m == 0 ? p : fmaf(-lam, p, sum);
-          s[m][r] = p * ((m == 0 ? dp[r] : -lam * dp[r]) - rows[(MAPS + m) * KEYS + i]);
+          const int i = m * KEYS + sub * 32 + 8 * g + 4 * half;
+          const f32x4 lse = *reinterpret_cast<const f32x4*>(rows + i), del = *reinterpret_cast<const f32x4*>(rows + MAPS * KEYS + i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            const float p = exp2_(fmaf(s[m][r], scale2, bias[r]) - lse[e]);
+            mix[r] = m == 0 ? p : fmaf(-lam, p, mix[r]);
+            s[m][r] = p * (m == 0 ? dp[r] - del[e] : fmaf(-lam, dp[r], -del[e]));
+          }
         }
-        mix[r] = sum;
-      }
 #pragma unroll
       for (int ks = 0; ks < 32 / M::KC; ++ks) {
         const Frag pf = M::pack(mix, ks);
@@ -304,7 +333,15 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(const AttnArgs 
       }
     }
   }
-  if (j >= a.Lk) return;                                          // keys from lengths[b] on get zeros
+  if (j >= a.Lk) return;
+  if (!mine) {                                                   // a key from lengths[b] on: zeros (its column has whatever its clamped place gave)
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int n = 0; n < DQ / 32; ++n) dk[m][n] = zero16();
+#pragma unroll
+    for (int n = 0; n < DV / 32; ++n) dv[n] = zero16();
+  }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     T* dst = static_cast<T*>(a.dk) + b * a.dks[0] + (int64_t)j * a.dks[1] + (int64_t)(MAPS * h + m) * a.dks[2];
@@ -385,11 +422,6 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
-static int ring_floats(const im2im_attention_desc* p) {
-  int n = 64;
-  while (n < window_floats(p->gh, p->gw)) n *= 2;
-  return n;
-}
 
 // images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, so their number (about 1024)
 // bounds that memory
@@ -411,9 +443,9 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
 }
 
 template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, int window, hipStream_t st) {
-  auto kern = attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS>;
+  auto kern = a.row4 ? attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, true> : attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, false>;
   const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 256 +
-                      (size_t)(BIAS ? 2 * WAVES * a.ring : 0) * 4 + (size_t)round64(window) * 4;
+                      (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8 + (size_t)round64(window + 4) * 4;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_q_kernel");
@@ -423,8 +455,8 @@ template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const Attn
   hipLaunchKernelGGL((attn_delta_kernel<T, MAPS>), dim3((unsigned)cdiv((int64_t)a.B * a.H * a.Lq, 16)), dim3(256), 0, st, a, delta);
   if (int rc = check_launch("attn_delta_kernel")) return rc;
   if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, window, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, window, st)) return rc;
-  auto kern = attn_bwd_kv_kernel<T, DQ, DV, MAPS>;
-  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 2 * MAPS * KEYS * 4 + (size_t)round64(window) * 4;
+  auto kern = a.row4 && a.q_start % 4 == 0 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, true> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, false>;
+  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 2 * MAPS * KEYS * 4 + (size_t)round64(window + 4) * 4;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_kv_kernel");
@@ -476,8 +508,8 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
   a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
-  a.ring = ring_floats(p);
   const int window = window_floats(p->gh, p->gw);
+  a.ring = round64(window);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, window, delta, st) : dispatch_bwd<float>(a, p->maps, window, delta, st)) return rc;
   double* line = reinterpret_cast<double*>(w + l.line);

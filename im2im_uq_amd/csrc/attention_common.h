@@ -24,6 +24,7 @@ struct AttnArgs {
   const int32_t* lengths;             // [B] or null
   const float* lam;                   // [H] (two maps)
   int B, Lq, Lk, H, d, dv, gw, line_len, line_off, q_start, nq, nk;
+  int row4;                           // any four tokens from a multiple of four on lie side by side in the grid
   float scale;                        // of the scores
   // forward
   void* out;                          // [B][Lq][H][dv]
@@ -39,7 +40,7 @@ struct AttnArgs {
   int64_t dqs[3], dks[3], dvs[3];
   float* line_part;                   // [nq * groups][H][line_len] or null
   float* dlam_part;                   // [nq * groups][H]
-  int groups, group_images, ring;     // ring: floats in one copy of the LDS accumulator (a power of two)
+  int groups, group_images, ring;     // ring: places in one copy of the LDS accumulator
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -99,6 +100,7 @@ template <typename T> __device__ __forceinline__ typename Mma<T>::Frag load_frag
 template <typename T> __host__ __device__ constexpr int padded(int d) { return d + 16 / (int)sizeof(T); }   // LDS row length: 16 rows' 16-byte reads on distinct banks
 
 __device__ __forceinline__ f32x16 zero16() { return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
+__device__ __forceinline__ f32x16 splat16(float v) { return f32x16{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
 __device__ __forceinline__ int mfma_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 __device__ __forceinline__ int grid_code(int t, int gw) { return (t / gw) * (2 * gw - 1) + t % gw; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -124,6 +126,22 @@ template <typename T, int D, int NR> __device__ __forceinline__ void stage_rows(
       u32x4 x = {0, 0, 0, 0};
       if (r < valid && c < d) x = *reinterpret_cast<const u32x4*>(src + r * stride + c);
       *reinterpret_cast<u32x4*>(dst + r * S + c) = x;
+    }
+  }
+}
+
+// the bias of a lane's 16 scores: places codes[row] + off of the window.  ROW4: four rows' codes are consecutive (rising or falling), one place
+// serves them; behind the last valid row that may reach three places over the window's end, values that the callers mask.
+template <bool ROW4, int STEP = 1> __device__ __forceinline__ void window_bias(float* bias, const float* win, const int* codes, int off, int half) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if constexpr (ROW4) {
+      const float* w = win + codes[8 * g + 4 * half] + off;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[4 * g + e] = w[STEP * e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[4 * g + e] = win[codes[8 * g + 4 * half + e] + off];
     }
   }
 }

@@ -40,12 +40,16 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------- forward
-// One workgroup: 128 queries (a wave has 32 of them as its columns), keys in tiles of 64 through LDS.
+// One workgroup: 128 queries (a wave has 32 of them as its columns), keys in tiles of 64 through LDS, a wave takes 32 of them at a time.
+// The running maximum follows the scores only where they pass it by more than 2^GROW: until then probabilities up to 2^GROW are as exact in
+// 32 bits and in bf16 as those up to 1, and the accumulators need no rescaling (a handful of times a row).
 // SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
 // result exact to about 2^-18: the backward's row sums D = dO . O are taken from it, and the table's gradient, a 32-bit sum with much
 // cancellation, would carry a rounding of P to bf16 (2^-9) in every D.
-template <typename T, int DQ, int DV, int MAPS, bool SAVE>
-__global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) {
+constexpr float GROW = 8.f;
+
+template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4>
+__global__ __launch_bounds__(64 * WAVES, MAPS * DV >= 256 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NB = DV / 32;
@@ -71,7 +75,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) 
   for (int m = 0; m < MAPS; ++m)
     load_row_frags<T, DQ>(qf[m], static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)min(i, i_last) * a.qs[1] + (int64_t)(MAPS * h + m) * a.qs[2],
                           mine, a.d, half);
-  float mx[MAPS], sum[MAPS];
+  float mx[MAPS], sum[MAPS];                                      // of this lane's keys (a row's other half is 32 lanes away)
   f32x16 o[MAPS][NB];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
@@ -100,12 +104,12 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) 
     __syncthreads();
     if (!busy) continue;
 
-    f32x16 s[MAPS][2];
-#pragma unroll
+#pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
+      if (sub * 32 >= valid) break;
       float bias[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) bias[r] = win[kc[sub * 32 + mfma_row(r, half)] + aoff];
+      window_bias<ROW4>(bias, win, kc + sub * 32, aoff, half);
+      f32x16 s[MAPS];
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
         f32x16 acc = zero16();
@@ -113,52 +117,44 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) 
         for (int c = 0; c < DQ / M::KC; ++c)
           acc = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], acc);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[m][sub][r] = fmaf(acc[r], scale2, bias[r]);
+        for (int r = 0; r < 16; ++r) s[m][r] = fmaf(acc[r], scale2, bias[r]);
       }
-    }
-    if (valid < KEYS) {
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+      if (valid < sub * 32 + 32) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (sub * 32 + mfma_row(r, half) >= valid)
 #pragma unroll
-            for (int m = 0; m < MAPS; ++m) s[m][sub][r] = -INFINITY;
-    }
+            for (int m = 0; m < MAPS; ++m) s[m][r] = -INFINITY;
+      }
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      float top = s[m][0][0];
+      for (int m = 0; m < MAPS; ++m) {
+        float top = s[m][0];
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[m][r]);
+        if (__any(top > mx[m] + GROW)) {
+          top = fmaxf(mx[m], fmaxf(top, __shfl_xor(top, 32)));
+          const float shrink = top == -INFINITY ? 1.f : exp2_(mx[m] - top);
+          mx[m] = top;
+          sum[m] *= shrink;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[m][sub][r]);
-      top = fmaxf(mx[m], fmaxf(top, __shfl_xor(top, 32)));
-      const float ref = top == -INFINITY ? 0.f : top;          // nothing but masks so far
-      const float shrink = exp2_(mx[m] - ref);
-      mx[m] = top;
-      float add = 0.f;
+          for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+            for (int r = 0; r < 16; ++r) o[m][n][r] *= shrink;
+        }
+        const float ref = mx[m] == -INFINITY ? 0.f : mx[m];      // nothing but masks so far
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[m][sub][r] = exp2_(s[m][sub][r] - ref);
-          add += s[m][sub][r];
+          s[m][r] = exp2_(s[m][r] - ref);
+          sum[m] += s[m][r];
         }
-      sum[m] = sum[m] * shrink + add;
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[m][n][r] *= shrink;
-    }
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+      }
 #pragma unroll
       for (int ks = 0; ks < 32 / M::KC; ++ks) {
         Frag pf[MAPS], pr[MAPS];
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
-          pf[m] = M::pack(s[m][sub], ks);
-          if (SAVE && sizeof(T) == 2) pr[m] = M::pack_rest(s[m][sub], pf[m], ks);
+          pf[m] = M::pack(s[m], ks);
+          if (SAVE && sizeof(T) == 2) pr[m] = M::pack_rest(s[m], pf[m], ks);
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -170,6 +166,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) 
           }
         }
       }
+    }
   }
 
   if (!busy) return;
@@ -226,36 +223,81 @@ __global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(const AttnArgs a) 
     }
 }
 
-// joins the parts of a row: 32 lanes for each row, four channels a lane
-template <typename T, int MAPS> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs a) {
-  const int64_t rows = (int64_t)a.B * a.H * a.Lq, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int c = (threadIdx.x & 31) * 4, i = (int)(row % a.Lq), bh = (int)(row / a.Lq), h = bh % a.H, b = bh / a.H;
+// joins the parts of a row: 32 lanes (four channels each) times G groups, which take the parts in turn.  Bound by the latency of its loads:
+// one group needs 40 us for 64 parts, eight need 7.
+template <typename T, int MAPS, int G> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs a) {
+  __shared__ float tops[8][MAPS], sums[8][MAPS];
+  __shared__ f32x4 parts[8][MAPS][32];
+  const int64_t rows = (int64_t)a.B * a.H * a.Lq, row = (int64_t)blockIdx.x * (8 / G) + (threadIdx.x >> 5) / G;
+  const int group = (threadIdx.x >> 5) % G, slot = (threadIdx.x >> 5) / G * G, l = threadIdx.x & 31, c = l * 4;
+  const bool mine = row < rows;
+  float top[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    top[m] = -INFINITY;
+    if (mine)
+      for (int s = group * 32 + l; s < a.splits; s += 32 * G) top[m] = fmaxf(top[m], a.part_ml[((s * rows + row) * MAPS + m) * 2]);
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) top[m] = fmaxf(top[m], __shfl_xor(top[m], x));
+    if (G > 1 && l == 0) tops[slot + group][m] = top[m];
+  }
+  if (G > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int g = 0; g < G; ++g) top[m] = fmaxf(top[m], tops[slot + g][m]);
+  }
+  float sum[MAPS];
+  f32x4 o[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    const float ref = top[m] == -INFINITY ? 0.f : top[m];
+    sum[m] = 0.f;
+    o[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (mine)
+#pragma unroll 4
+      for (int s = group; s < a.splits; s += G) {
+        const int64_t at = (s * rows + row) * MAPS + m;
+        const float w = exp2_(a.part_ml[at * 2] - ref);
+        sum[m] += w * a.part_ml[at * 2 + 1];
+        if (c < a.dv) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * a.dv + c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[m][e] = fmaf(w, x[e], o[m][e]);
+        }
+      }
+    if (G > 1) {
+      if (l == 0) sums[slot + group][m] = sum[m];
+      parts[slot + group][m][l] = o[m];
+    }
+  }
+  if (G > 1) {
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+      for (int g = 1; g < G; ++g) {
+        sum[m] += sums[slot + g][m];
+        const f32x4 x = parts[slot + g][m][l];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[m][e] += x[e];
+      }
+  }
+  if (!mine) return;
+  const int i = (int)(row % a.Lq), bh = (int)(row / a.Lq), h = bh % a.H, b = bh / a.H;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[((s * rows + row) * MAPS + m) * 2]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-      const int64_t at = (s * rows + row) * MAPS + m;
-      const float w = exp2_(a.part_ml[at * 2] - ref);
-      sum += w * a.part_ml[at * 2 + 1];
-      if (c < a.dv) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * a.dv + c);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += w * x[e];
-      }
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    if (a.lse && c == 0) a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum > 0.f ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+    const float inv = sum[m] > 0.f ? 1.f / sum[m] : 0.f;
+    if (a.lse && l == 0) a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum[m] > 0.f ? top[m] + __builtin_amdgcn_logf(sum[m]) : INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o[e] *= inv;
-      v[e] += m == 0 ? o[e] : -a.lam[h] * o[e];
+      o[m][e] *= inv;
+      v[e] += m == 0 ? o[m][e] : -a.lam[h] * o[m][e];
     }
-    if (a.osave && c < a.dv) store4(a.osave + (row * MAPS + m) * a.dv + c, o[0], o[1], o[2], o[3]);
+    if (a.osave && c < a.dv) store4(a.osave + (row * MAPS + m) * a.dv + c, o[m][0], o[m][1], o[m][2], o[m][3]);
   }
   if (c < a.dv) store4(static_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv + c, v[0], v[1], v[2], v[3]);
 }
@@ -306,6 +348,7 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   a->line_len = (2 * p->gh - 1) * (2 * p->gw - 1);
   a->line_off = (p->gh - 1) * (2 * p->gw - 1) + p->gw - 1;
   a->q_start = p->q_start;
+  a->row4 = p->gh == 1 || p->gw % 4 == 0;
   a->nq = (int)cdiv(p->Lq, ROWS);
   a->nk = (int)cdiv(p->Lk, ROWS);
   a->scale = p->scale;
@@ -324,13 +367,15 @@ static int key_splits(const AttnArgs& a) {
 }
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, int window, hipStream_t st) {
-  auto kern = attn_fwd_kernel<T, DQ, DV, MAPS, SAVE>;
-  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + (size_t)round64(window) * 4;
+  auto kern = a.row4 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, true> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, false>;
+  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + (size_t)round64(window + 4) * 4;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nq * a.splits)), dim3(64 * WAVES), smem, st, a);
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
   if (a.splits > 1) {
-    hipLaunchKernelGGL((attn_combine_kernel<T, MAPS>), dim3((unsigned)cdiv((int64_t)a.B * a.H * a.Lq, 8)), dim3(256), 0, st, a);
+    const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+    if (a.splits >= 8) hipLaunchKernelGGL((attn_combine_kernel<T, MAPS, 8>), dim3((unsigned)rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_combine_kernel<T, MAPS, 1>), dim3((unsigned)cdiv(rows, 8)), dim3(256), 0, st, a);
     return check_launch("attn_combine_kernel");
   }
   return IM2IM_OK;

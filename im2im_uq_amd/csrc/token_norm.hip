@@ -302,18 +302,24 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_gate_bwd_kernel(co
   }
 }
 
-// [blocks][5][C] -> the weights' gradients: 64 channels a workgroup, the blocks over its four waves
+// [blocks][5][C] -> the weights' gradients: 64 channels a workgroup, the blocks dealt to its 16 waves (with four waves its chains of loads took
+// 33 us at 512 blocks, more than the pass over the rows of a small call)
 struct NormSumArgs { const float* part; float* out[5]; int blocks, C; };
-__global__ __launch_bounds__(256) void norm_gate_sum_kernel(const NormSumArgs a) {
-  __shared__ double part[4][64];
-  const int k = blockIdx.y, c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void norm_gate_sum_kernel(const NormSumArgs a) {
+  __shared__ double part[16][64];
+  const int k = blockIdx.y, l = threadIdx.x & 63, c = blockIdx.x * 64 + l, wave = threadIdx.x >> 6;
   if (!a.out[k]) return;
   double acc = 0.0;
   if (c < a.C)
-    for (int b = wave; b < a.blocks; b += 4) acc += (double)a.part[((int64_t)b * 5 + k) * a.C + c];
-  part[wave][threadIdx.x & 63] = acc;
+#pragma unroll 8
+    for (int b = wave; b < a.blocks; b += 16) acc += (double)a.part[((int64_t)b * 5 + k) * a.C + c];
+  part[wave][l] = acc;
   __syncthreads();
-  if (wave == 0 && c < a.C) a.out[k][c] = (float)(part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x]);
+  if (wave == 0 && c < a.C) {
+#pragma unroll
+    for (int w = 1; w < 16; ++w) acc += part[w][l];
+    a.out[k][c] = (float)acc;
+  }
 }
 
 // -------------------------------------------------------------------------------------------------------------------- host
@@ -435,6 +441,6 @@ extern "C" int im2im_norm_gate_bwd(const im2im_norm_gate_desc* p, const void* dy
   NormSumArgs s = {};
   s.part = a.part; s.blocks = (int)bwd_blocks(a.rows, a.C); s.C = a.C;
   s.out[0] = dscale; s.out[1] = dpost_weight; s.out[2] = dpost_bias; s.out[3] = dpre_weight; s.out[4] = dpre_bias;
-  hipLaunchKernelGGL(norm_gate_sum_kernel, dim3((unsigned)cdiv(a.C, 64), 5), dim3(256), 0, st, s);
+  hipLaunchKernelGGL(norm_gate_sum_kernel, dim3((unsigned)cdiv(a.C, 64), 5), dim3(1024), 0, st, s);
   return check_launch("norm_gate_sum_kernel");
 }
