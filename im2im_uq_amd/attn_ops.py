@@ -75,212 +75,226 @@ def _parameter(name, t, shape, device):
         _fail(f"{name}: expected fp32 {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
-def _rows16(t):
-    """`t` with its last index dense and every row at 16 bytes, as the kernels read it (a copy only where it is not)"""
-    e = t.element_size()
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1])
-    return t if ok else _dense16(t)
-
-
 def _dense16(t):
+    """`t` dense and at 16 bytes"""
     t = t if t.is_contiguous() else t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-class _on:
-    """the operands' device as the current one, for the launches (torch.cuda.device only where it is another)"""
-    __slots__ = ("idx", "guard")
+def _rows16(t):
+    """`t` with its last index dense and every row at 16 bytes, as the kernels read it (a copy only where it is not)"""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():                                # heads are multiples of 16 bytes long
+            return t
+        e, strides = t.element_size(), t.stride()
+        if strides[-1] == 1 and all(s * e % 16 == 0 for s in strides[:-1]):
+            return t
+    return _dense16(t)
 
-    def __init__(self, device):
-        self.idx = device.index
 
-    def __enter__(self):
-        self.guard = None
-        if self.idx != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.idx)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _guard(device):
+    """the operands' device made the current one for the launches; None where it is already"""
+    if device.index == torch._C._cuda_getDevice():
+        return None
+    guard = torch.cuda.device(device.index)
+    guard.__enter__()
+    return guard
 
 
 class _Plan:
-    """the whole numbers of a call"""
-    __slots__ = ("heads", "d", "maps", "gh", "gw", "my", "mx", "q_start", "scale")
+    """what a call is, beside its tensors: settled once for each combination of sizes (plain numbers only)"""
+    __slots__ = ("heads", "d", "maps", "desc", "sizes", "table_shape", "thr", "out_shape", "save", "fwd_ws", "bwd_ws", "line_at", "lse_at", "map_at")
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distance, q_start, scale):
+    if dtype not in _DT:
+        _fail(f"q, k, v: fp32 or bf16, got {dtype}")
+    if not len(q_shape) == len(k_shape) == len(v_shape) == 4:
+        _fail(f"q, k, v: expected [batch, tokens, heads, channels], got {list(q_shape)}, {list(k_shape)}, {list(v_shape)}")
+    b, lq, hm, d = q_shape
+    lk, heads = k_shape[1], v_shape[2]
+    if hm != heads * maps or tuple(k_shape) != (b, lk, hm, d) or tuple(v_shape) != (b, lk, heads, d * maps):
+        _fail(f"shapes do not belong together: q {list(q_shape)}, k {list(k_shape)}, v {list(v_shape)} with {maps} map(s): k [batch, keys, "
+              f"{maps} * heads, D], v [batch, keys, heads, {maps} * D]")
+    if heads < 1 or d < 8 or d % 8 or d * maps > 128:
+        _fail(f"head size: a multiple of 8 up to {128 // maps} with {maps} map(s), got {d} ({heads} heads)")
+    try:
+        gh, gw = (int(x) for x in grid)
+        my, mx = (int(x) for x in max_distance) if isinstance(max_distance, tuple) else (int(max_distance),) * 2
+    except (TypeError, ValueError):
+        _fail(f"grid = (height, width) and max_distance = a number or (vertical, horizontal), got {grid!r}, {max_distance!r}")
+    if gh < 1 or gw < 1 or gh * gw > 1 << 24 or (gh > 1 and gw > MAX_GRID_WIDTH):
+        _fail(f"grid {grid}: at least 1 x 1, at most 2**24 tokens, and at most {MAX_GRID_WIDTH} wide unless it is one row")
+    if lk > gh * gw:
+        _fail(f"{lk} keys do not fit the grid {grid}")
+    if q_start < 0 or q_start + lq > gh * gw:
+        _fail(f"queries {q_start} .. {q_start + lq - 1} are not tokens of the grid {grid}")
+    if len(table_shape) != 3 or table_shape[2] != heads:
+        _fail(f"table: expected fp32 [vertical buckets, horizontal buckets, {heads}], got {list(table_shape)}")
+    p = _Plan()
+    p.thr = _thresholds_arg(table_shape[0], my), _thresholds_arg(table_shape[1], mx)
+    p.heads, p.d, p.maps, p.table_shape, p.out_shape = heads, d, maps, tuple(table_shape), (b, lq, heads, d * maps)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        _fail(f"scale must be finite, got {scale}")
+    if b * lq and lk == 0:
+        _fail("k, v: no keys (lengths may be 0, the tensors not)")
+    p.desc = None
+    if b * lq == 0:
+        return p
+    # the description with the pointers left open, and the sizes that follow from it
+    t = p.desc = AttentionDesc()
+    t.B, t.Lq, t.Lk, t.H, t.D, t.maps, t.gh, t.gw, t.q_start, t.dtype, t.scale = b, lq, lk, heads, d, maps, gh, gw, q_start, _DT[dtype], scale
+    t.q = t.k = t.v = t.line = t.lam = 16
+    p.fwd_ws = lib.im2im_attention_fwd_workspace_bytes(ctypes.byref(t))
+    p.bwd_ws = [lib.im2im_attention_bwd_workspace_bytes(ctypes.byref(t), w) for w in (0, 1)]
+    if p.fwd_ws < 0 or min(p.bwd_ws) < 0:
+        check(-1, "im2im_attention_fwd")
+    # one buffer for the bias of every displacement and what the backward needs; places in floats, at 16 bytes
+    up = lambda n: (n + 3) // 4 * 4  # noqa: E731
+    p.line_at = 0
+    p.lse_at = up(heads * (2 * gh - 1) * (2 * gw - 1))
+    p.map_at = p.lse_at + up(b * heads * maps * lq)
+    p.save = p.map_at + b * heads * lq * maps * d * maps
+    return p
 
 
 def _describe(plan, q, k, v, line, lengths, lam):
-    p = AttentionDesc()
-    p.q, p.k, p.v, p.line = q.data_ptr(), k.data_ptr(), v.data_ptr(), line.data_ptr()
-    p.lengths = None if lengths is None else lengths.data_ptr()
-    p.lam = None if lam is None else lam.data_ptr()
+    p = AttentionDesc.from_buffer_copy(plan.desc)
+    p.q, p.k, p.v, p.line = q.data_ptr(), k.data_ptr(), v.data_ptr(), line
+    p.lengths, p.lam = _ptr(lengths), _ptr(lam)
     p.q_stride[:], p.k_stride[:], p.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    p.B, p.Lq, p.Lk, p.H, p.D, p.maps = q.shape[0], q.shape[1], k.shape[1], plan.heads, plan.d, plan.maps
-    p.gh, p.gw, p.q_start, p.dtype, p.scale = plan.gh, plan.gw, plan.q_start, _DT[q.dtype], plan.scale
     return p
 
 
 def _forward(plan, q, k, v, table, lam, lengths, keep):
-    """(out, line, lse, map_out); the last two only with `keep`"""
+    """(out, saved): the buffer of the plan's line, log-sums and map results"""
     dev = q.device
-    b, lq, h, maps = q.shape[0], q.shape[1], plan.heads, plan.maps
-    dv = plan.d * maps
-    out = torch.empty((b, lq, h, dv), dtype=q.dtype, device=dev)
-    ny, nx = table.shape[0], table.shape[1]
-    line = torch.empty((h, (2 * plan.gh - 1) * (2 * plan.gw - 1)), dtype=F32, device=dev)
-    lse = torch.empty((b * h, maps, lq), dtype=F32, device=dev) if keep else None
-    map_out = torch.empty((b * h, lq, maps, dv), dtype=F32, device=dev) if keep else None
-    with _on(dev) as stream:
-        check(lib.im2im_relpos_line(table.data_ptr(), ny, nx, h, _thresholds_arg(ny, plan.my), _thresholds_arg(nx, plan.mx), plan.gh, plan.gw,
-                                    line.data_ptr(), stream), "im2im_relpos_line")
+    out = torch.empty(plan.out_shape, dtype=q.dtype, device=dev)
+    saved = torch.empty(plan.save if keep else plan.lse_at, dtype=F32, device=dev)
+    ws = torch.empty(plan.fwd_ws, dtype=torch.uint8, device=dev) if plan.fwd_ws else None
+    guard = _guard(dev)
+    try:
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        line, t, shape = saved.data_ptr(), plan.desc, plan.table_shape
+        check(lib.im2im_relpos_line(table.data_ptr(), shape[0], shape[1], t.H, plan.thr[0], plan.thr[1], t.gh, t.gw, line, stream), "im2im_relpos_line")
         p = _describe(plan, q, k, v, line, lengths, lam)
-        n = lib.im2im_attention_fwd_workspace_bytes(ctypes.byref(p))
-        if n < 0:
-            check(-1, "im2im_attention_fwd")
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), lse.data_ptr() if keep else None, map_out.data_ptr() if keep else None,
-                                      ws.data_ptr() if n else None, n, stream), "im2im_attention_fwd")
-    return out, line, lse, map_out
+        check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), line + 4 * plan.lse_at if keep else None, line + 4 * plan.map_at if keep else None,
+                                      _ptr(ws), plan.fwd_ws, stream), "im2im_attention_fwd")
+    finally:
+        if guard is not None:
+            guard.__exit__(None, None, None)
+    return out, saved
 
 
-def _backward(plan, q, k, v, table_shape, line, lam, lengths, lse, map_out, dout, dq, dk, dv, want_table):
+def _backward(plan, q, k, v, saved, lam, lengths, dout, dq, dk, dv, want_table):
     """fills dq, dk, dv ([B, L, heads, D] views); returns (dtable | None, dlam | None)"""
     dev = q.device
     dout = _dense16(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-    dtable = torch.empty(table_shape, dtype=F32, device=dev) if want_table else None
+    dtable = torch.empty(plan.table_shape, dtype=F32, device=dev) if want_table else None
     dlam = torch.empty(plan.heads, dtype=F32, device=dev) if plan.maps == 2 else None
-    with _on(dev) as stream:
-        p = _describe(plan, q, k, v, line, lengths, lam)
-        g = AttentionGrads()
-        g.dout, g.lse, g.map_out = dout.data_ptr(), lse.data_ptr(), map_out.data_ptr()
-        g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        g.dq_stride[:], g.dk_stride[:], g.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
-        g.dtable, g.dlam = dtable.data_ptr() if want_table else None, dlam.data_ptr() if dlam is not None else None
-        ty, tx = _thresholds_arg(table_shape[0], plan.my), _thresholds_arg(table_shape[1], plan.mx)
-        g.thr_y, g.thr_x = ctypes.cast(ty, ctypes.c_void_p), ctypes.cast(tx, ctypes.c_void_p)
-        g.ny, g.nx = table_shape[0], table_shape[1]
-        n = lib.im2im_attention_bwd_workspace_bytes(ctypes.byref(p), int(want_table))
-        if n < 0:
-            check(-1, "im2im_attention_bwd")
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        check(lib.im2im_attention_bwd(ctypes.byref(p), ctypes.byref(g), ws.data_ptr(), n, stream), "im2im_attention_bwd")
+    n = plan.bwd_ws[want_table]
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    line = saved.data_ptr()
+    g = AttentionGrads(dout.data_ptr(), line + 4 * plan.lse_at, line + 4 * plan.map_at, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(dlam))
+    g.dq_stride[:], g.dk_stride[:], g.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+    if want_table:
+        g.ny, g.nx = plan.table_shape[:2]
+        g.thr_y, g.thr_x = (ctypes.cast(t, ctypes.c_void_p) for t in plan.thr)
+    p = _describe(plan, q, k, v, line, lengths, lam)
+    guard = _guard(dev)
+    try:
+        check(lib.im2im_attention_bwd(ctypes.byref(p), ctypes.byref(g), ws.data_ptr(), n, torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_attention_bwd")
+    finally:
+        if guard is not None:
+            guard.__exit__(None, None, None)
     return dtable, dlam
 
 
 class _GridAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, lam, lengths, plan, keep):
-        table, lam = table.contiguous(), None if lam is None else lam.contiguous()
-        out, line, lse, map_out = _forward(plan, q, k, v, table, lam, lengths, keep)
-        if keep:
-            ctx.plan, ctx.table_shape = plan, tuple(table.shape)
-            ctx.save_for_backward(q, k, v, line, lam, lengths, lse, map_out)
+    def forward(ctx, q, k, v, table, lam, lengths, plan):
+        out, saved = _forward(plan, q, k, v, table.contiguous(), None if lam is None else lam.contiguous(), lengths, True)
+        ctx.plan = plan
+        ctx.save_for_backward(q, k, v, lam, lengths, saved)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, line, lam, lengths, lse, map_out = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dtable, dlam = _backward(ctx.plan, q, k, v, ctx.table_shape, line, lam, lengths, lse, map_out, dout, dq, dk, dv, ctx.needs_input_grad[3])
-        return dq, dk, dv, dtable, dlam, None, None, None
+        q, k, v, lam, lengths, saved = ctx.saved_tensors
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        dtable, dlam = _backward(ctx.plan, q, k, v, saved, None if lam is None else lam.contiguous(), lengths, dout, dq, dk, dv, ctx.needs_input_grad[3])
+        return dq, dk, dv, dtable, dlam, None, None
 
 
 class _GridSelfAttention(torch.autograd.Function):
     """q, k and v side by side in one tensor: their gradients leave in one tensor too, without the copies that three slices would cost"""
 
     @staticmethod
-    def forward(ctx, qkv, table, lam, plan, keep):
-        table, lam = table.contiguous(), None if lam is None else lam.contiguous()
+    def forward(ctx, qkv, table, lam, plan):
         qkv = _rows16(qkv)
-        out, line, lse, map_out = _forward(plan, *_split_qkv(qkv, plan), table, lam, None, keep)
-        if keep:
-            ctx.plan, ctx.table_shape = plan, tuple(table.shape)
-            ctx.save_for_backward(qkv, line, lam, lse, map_out)
+        out, saved = _forward(plan, *_split_qkv(qkv, plan), table.contiguous(), None if lam is None else lam.contiguous(), None, True)
+        ctx.plan = plan
+        ctx.save_for_backward(qkv, lam, saved)
         return out.view(out.shape[0], out.shape[1], -1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, line, lam, lse, map_out = ctx.saved_tensors
+        qkv, lam, saved = ctx.saved_tensors
         plan = ctx.plan
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        dout = dout.reshape(qkv.shape[0], qkv.shape[1], plan.heads, plan.d * plan.maps)
-        dtable, dlam = _backward(plan, *_split_qkv(qkv, plan), ctx.table_shape, line, lam, None, lse, map_out, dout, *_split_qkv(dqkv, plan),
-                                 ctx.needs_input_grad[1])
-        return dqkv, dtable, dlam, None, None
+        dtable, dlam = _backward(plan, *_split_qkv(qkv, plan), saved, None if lam is None else lam.contiguous(), None, dout.reshape(plan.out_shape),
+                                 *_split_qkv(dqkv, plan), ctx.needs_input_grad[1])
+        return dqkv, dtable, dlam, None
 
 
 def _split_qkv(t, plan):
-    b, n, c3 = t.shape
-    c = c3 // 3
-    q, k, v = t[..., :c], t[..., c:2 * c], t[..., 2 * c:]
+    c = t.shape[2] // 3
     maps, h, d = plan.maps, plan.heads, plan.d
-    return q.unflatten(2, (h * maps, d)), k.unflatten(2, (h * maps, d)), v.unflatten(2, (h, d * maps))
+    return tuple(t[..., i * c:(i + 1) * c].unflatten(2, (h * maps, d) if i < 2 else (h, d * maps)) for i in range(3))
 
 
-def _make_plan(maps, heads, d, dtype, table, lam, grid, max_distance, lk, lq, q_start, scale, device):
-    if dtype not in _DT:
-        _fail(f"q, k, v: fp32 or bf16, got {dtype}")
-    if heads < 1 or d < 8 or d % 8 or d * maps > 128:
-        _fail(f"head size: a multiple of 8 up to {128 // maps} with {maps} map(s), got {d} ({heads} heads)")
-    p = _Plan()
-    try:
-        p.gh, p.gw = (int(x) for x in grid)
-        p.my, p.mx = (int(x) for x in max_distance) if isinstance(max_distance, (tuple, list)) else (int(max_distance),) * 2
-    except (TypeError, ValueError):
-        _fail(f"grid = (height, width) and max_distance = a number or (vertical, horizontal), got {grid!r}, {max_distance!r}")
-    if p.gh < 1 or p.gw < 1 or p.gh * p.gw > 1 << 24 or (p.gh > 1 and p.gw > MAX_GRID_WIDTH):
-        _fail(f"grid {grid}: at least 1 x 1, at most 2**24 tokens, and at most {MAX_GRID_WIDTH} wide unless it is one row")
-    if lk > p.gh * p.gw:
-        _fail(f"{lk} keys do not fit the grid {grid}")
-    if q_start < 0 or q_start + lq > p.gh * p.gw:
-        _fail(f"queries {q_start} .. {q_start + lq - 1} are not tokens of the grid {grid}")
-    _on_gpu("table", table, device)
-    if table.dtype != F32 or table.dim() != 3 or table.shape[2] != heads:
-        _fail(f"table: expected fp32 [vertical buckets, horizontal buckets, {heads}], got {table.dtype} {list(table.shape)}")
-    bucket_thresholds(table.shape[0], p.my)
-    bucket_thresholds(table.shape[1], p.mx)
-    if maps == 2:
-        _parameter("lam", lam, (heads,), device)
-    p.heads, p.d, p.maps, p.q_start = heads, d, maps, q_start
-    p.scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(p.scale):
-        _fail(f"scale must be finite, got {scale}")
-    return p
+def _numbers(x):
+    return tuple(x) if isinstance(x, list) else x
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, scale):
     _on_gpu("q", q)
-    _on_gpu("k", k, q.device)
-    _on_gpu("v", v, q.device)
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        _fail(f"q, k, v: expected [batch, tokens, heads, channels], got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    dev = q.device
+    _on_gpu("k", k, dev)
+    _on_gpu("v", v, dev)
+    _on_gpu("table", table, dev)
     if not q.dtype == k.dtype == v.dtype:
         _fail(f"q, k, v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
-    b, lq, hm, d = q.shape
-    lk, h = k.shape[1], v.shape[2]
-    if hm != h * maps or tuple(k.shape) != (b, lk, hm, d) or tuple(v.shape) != (b, lk, h, d * maps):
-        _fail(f"shapes do not belong together: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} with {maps} map(s): k [batch, keys, "
-              f"{maps} * heads, D], v [batch, keys, heads, {maps} * D]")
-    plan = _make_plan(maps, h, d, q.dtype, table, lam, grid, max_distance, lk, lq, q_start, scale, q.device)
+    if table.dtype != F32:
+        _fail(f"table: expected fp32, got {table.dtype}")
+    plan = _plan(maps, q.shape, k.shape, v.shape, q.dtype, table.shape, _numbers(grid), _numbers(max_distance), q_start, scale)
+    if maps == 2:
+        _parameter("lam", lam, (plan.heads,), dev)
     if lengths is not None:
-        _on_gpu("lengths", lengths, q.device)
-        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (b,):
-            _fail(f"lengths: expected int32 [{b}], got {lengths.dtype} {list(lengths.shape)}")
+        _on_gpu("lengths", lengths, dev)
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],):
+            _fail(f"lengths: expected int32 [{q.shape[0]}], got {lengths.dtype} {list(lengths.shape)}")
         lengths = lengths.contiguous()
-    needs = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad
-                                         or (lam is not None and lam.requires_grad))
-    if b * lq == 0:                                          # nothing is asked for
-        return v.new_empty((b, lq, h, d * maps)) + 0 * q.sum() if needs else v.new_empty((b, lq, h, d * maps))
-    if lk == 0:
-        _fail("k, v: no keys (lengths may be 0, the tensors not)")
+    needs = _needs_grad(q, k, v, table, lam)
+    if plan.desc is None:                                    # nothing is asked for
+        out = v.new_empty(plan.out_shape)
+        return out + 0 * q.sum() if needs else out
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    if not needs:
-        return _forward(plan, q, k, v, table.contiguous(), None if lam is None else lam.contiguous(), lengths, False)[0]
-    return _GridAttention.apply(q, k, v, table, lam, lengths, plan, True)
+    if needs:
+        return _GridAttention.apply(q, k, v, table, lam, lengths, plan)
+    return _forward(plan, q, k, v, table.contiguous(), None if lam is None else lam.contiguous(), lengths, False)[0]
 
 
 def grid_attention(q, k, v, table, grid, max_distance=64, lengths=None, q_start=0, scale=None):
@@ -315,16 +329,25 @@ def grid_self_attention(qkv, heads, table, grid, lam=None, max_distance=64, scal
     and v side by side, C = heads * D (differential: C = heads * 2 * D), and so does its gradient.  Returns [B, height * width, C]."""
     _on_gpu("qkv", qkv)
     maps = 1 if lam is None else 2
-    if qkv.dim() != 3 or heads < 1 or qkv.shape[2] % (3 * heads * maps):
+    if qkv.dim() != 3 or not isinstance(heads, int) or heads < 1 or qkv.shape[2] % (3 * heads * maps):
         _fail(f"qkv: expected [batch, tokens, 3 * C] with C a multiple of {heads} heads x {maps} map(s), got {list(qkv.shape)}")
+    _on_gpu("table", table, qkv.device)
+    if table.dtype != F32:
+        _fail(f"table: expected fp32, got {table.dtype}")
+    if lam is not None:
+        _parameter("lam", lam, (heads,), qkv.device)
     b, n, c3 = qkv.shape
-    plan = _make_plan(maps, heads, c3 // (3 * heads * maps), qkv.dtype, table, lam, grid, max_distance, n, n, 0, scale, qkv.device)
-    if n != plan.gh * plan.gw:
+    d = c3 // (3 * heads * maps)
+    shape, grid = (b, n, heads * maps, d), _numbers(grid)
+    plan = _plan(maps, shape, shape, (b, n, heads, d * maps), qkv.dtype, table.shape, grid, _numbers(max_distance), 0, scale)
+    if n != int(grid[0]) * int(grid[1]):
         _fail(f"{n} tokens are not the grid {grid}")
-    if b == 0:
+    if plan.desc is None:
         return qkv[..., :c3 // 3]
-    keep = torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad or (lam is not None and lam.requires_grad))
-    return _GridSelfAttention.apply(qkv, table, lam, plan, keep)
+    if _needs_grad(qkv, table, lam):
+        return _GridSelfAttention.apply(qkv, table, lam, plan)
+    out = _forward(plan, *_split_qkv(_rows16(qkv), plan), table.contiguous(), None if lam is None else lam.contiguous(), None, False)[0]
+    return out.view(b, n, c3 // 3)
 
 
 # ---------------------------------------------------------------------------------------------------------------------- norms
@@ -335,6 +358,8 @@ class _Seam:
 
 def _rows_of(t, shape):
     """`t` as [rows, C] with dense channels and one stride between its rows, and that stride (a copy only where there is none)"""
+    if t.is_contiguous():
+        return t, shape[-1]
     if t.stride(-1) == 1 or shape[-1] == 1:
         stride, size, ok = None, 1, True
         for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
@@ -349,15 +374,8 @@ def _rows_of(t, shape):
 
 
 def _seam_desc(s, x, f, gate, params):
-    p = NormGateDesc()
-    for name, t in (("x", x), ("f", f), ("gate", gate)):
-        if t is not None:
-            t, stride = t
-            setattr(p, name, t.data_ptr())
-            setattr(p, name + "_stride", stride)
-    p.scale, p.post_weight, p.post_bias, p.pre_weight, p.pre_bias = (None if t is None else t.data_ptr() for t in params)
-    p.rows, p.C, p.norm, p.dtype, p.eps = s.rows, s.c, s.norm, _DT[x[0].dtype], s.eps
-    return p
+    rows = [(None, 0) if t is None else (t[0].data_ptr(), t[1]) for t in (x, f, gate)]
+    return NormGateDesc(*(r[0] for r in rows), *(_ptr(t) for t in params), s.rows, *(r[1] for r in rows), s.c, s.norm, _DT[x[0].dtype], s.eps)
 
 
 def _seam_forward(s, x, f, gate, params):
@@ -366,9 +384,13 @@ def _seam_forward(s, x, f, gate, params):
     dev, dt = x[0].device, x[0].dtype
     y = torch.empty(s.shape, dtype=dt, device=dev) if f is not None else None
     h = torch.empty(s.shape, dtype=dt, device=dev) if params[3] is not None else None
-    with _on(dev) as stream:
-        check(lib.im2im_norm_gate_fwd(ctypes.byref(_seam_desc(s, x, f, gate, params)), None if y is None else y.data_ptr(),
-                                      None if h is None else h.data_ptr(), stream), "im2im_norm_gate_fwd")
+    guard = _guard(dev)
+    try:
+        check(lib.im2im_norm_gate_fwd(ctypes.byref(_seam_desc(s, x, f, gate, params)), _ptr(y), _ptr(h), torch._C._cuda_getCurrentRawStream(dev.index)),
+              "im2im_norm_gate_fwd")
+    finally:
+        if guard is not None:
+            guard.__exit__(None, None, None)
     return y, h
 
 
@@ -397,13 +419,16 @@ class _NormGate(torch.autograd.Function):
         want = [t is not None and n for t, n in zip(params, need[3:])]
         sums = [torch.empty(s.c, dtype=F32, device=dev) if w and (i < 3 or dh is not None) else None for i, w in enumerate(want)]
         params = [None if t is None else _dense16(t) for t in params]
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        with _on(dev) as stream:
-            n = lib.im2im_norm_gate_bwd_workspace_bytes(s.rows, s.c)
-            ws = torch.empty(n, dtype=torch.uint8, device=dev)
-            desc = _seam_desc(s, *(None if t is None else _rows_of(t, s.shape) for t in (x, f, gate)), params)
-            check(lib.im2im_norm_gate_bwd(ctypes.byref(desc), ptr(dy), ptr(dh), *(ptr(t) for t in rows), *(ptr(t) for t in sums), ws.data_ptr(), n,
-                                          stream), "im2im_norm_gate_bwd")
+        n = lib.im2im_norm_gate_bwd_workspace_bytes(s.rows, s.c)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        desc = _seam_desc(s, *(None if t is None else _rows_of(t, s.shape) for t in (x, f, gate)), params)
+        guard = _guard(dev)
+        try:
+            check(lib.im2im_norm_gate_bwd(ctypes.byref(desc), _ptr(dy), _ptr(dh), *map(_ptr, rows), *map(_ptr, sums), ws.data_ptr(), n,
+                                          torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_norm_gate_bwd")
+        finally:
+            if guard is not None:
+                guard.__exit__(None, None, None)
         sums = [torch.zeros(s.c, dtype=F32, device=dev) if w and t is None else t for w, t in zip(want, sums)]
         return (None, *rows, *sums)
 

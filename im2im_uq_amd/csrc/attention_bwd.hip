@@ -1,37 +1,11 @@
 // Grid attention, backward.  With P_m the softmax maps, A = P_1 (- lam P_2) and dP = dO V^T:
 //   dV = A^T dO,   dS_1 = P_1 o (dP - D_1),   dS_2 = P_2 o (-lam dP - D_2),   D_m = rowsum(P_m o dP_m) = dO . O_m (times -lam for m = 2),
 //   dQ_m = scale dS_m K_m,   dK_m = scale dS_m^T Q_m,   dbias(j - i) = sum of dS_1 + dS_2,   dlam = -sum P_2 o dP.
-// Two passes, each with its own tile of the scores (computed again from Q, K and the saved log-sums): queries' gradients and the bias in
-// one, keys' and values' gradients in the other.  No global atomics: every sum has one order.
+// Two passes, each with its own tile of the scores (computed again from Q, K and the saved log-sums): D, the queries' gradients and the bias
+// in one, the keys' and values' gradients in the other.  No global atomics: every sum has one order.
 #include "attention_common.h"
 
 namespace im2im {
-
-// D of every row, 16 lanes a row: reads dO and the saved map results once (bound by that)
-template <typename T, int MAPS> __global__ __launch_bounds__(256) void attn_delta_kernel(const AttnArgs a, float* delta) {
-  const int64_t rows = (int64_t)a.B * a.H * a.Lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;
-  const int i = (int)(row % a.Lq), bh = (int)(row / a.Lq), h = bh % a.H, b = bh / a.H, l = threadIdx.x & 15;
-  const T* g = static_cast<const T*>(a.dout) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv;
-  float acc[MAPS] = {};
-  for (int c = l * 4; c < a.dv; c += 64) {
-    float gv[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) gv[e] = to_float(g[c + e]);
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.osave + (row * MAPS + m) * a.dv + c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m] = fmaf(gv[e], x[e], acc[m]);
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < MAPS; ++m) {
-#pragma unroll
-    for (int s = 8; s >= 1; s >>= 1) acc[m] += __shfl_xor(acc[m], s);
-    if (l == 0) delta[((int64_t)bh * MAPS + m) * a.Lq + i] = m == 0 ? acc[m] : -a.lam[h] * acc[m];
-  }
-}
 
 // a place of the ring, summed over its copies in their order, and zeros in its place
 template <bool ROW4> __device__ __forceinline__ double take_place(double* ring, unsigned place, unsigned size) {
@@ -56,17 +30,15 @@ template <bool ROW4> __device__ __forceinline__ double take_place(double* ring, 
 // that the following tiles cannot reach any more are summed over the copies and written, each once.  The copies are 64-bit:
 // ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 3xx us at 78 images of 20 x 20, 8 x 64.
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4>
-__global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
+  using St = Stage<T, DQ, DV, MAPS>;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NBUF = buffers<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* Ks = reinterpret_cast<T*>(smem);
-  T* Vs = Ks + MAPS * KEYS * SQ;
-  int* kc = reinterpret_cast<int*>(Vs + KEYS * SV);
-  float* red = reinterpret_cast<float*>(kc + KEYS);              // [WAVES]
-  double* ring = reinterpret_cast<double*>(red + 64);            // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
-  float* win = reinterpret_cast<float*>(ring + (BIAS ? 2 * WAVES * (a.ring + 4) : 0));
+  const size_t buffer = St::TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
+  double* ring = reinterpret_cast<double*>(smem + NBUF * buffer);          // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
+  __shared__ float red[WAVES];
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, gh_ = lin / a.nq, h = gh_ % a.H, group = gh_ / a.H;
   const int slot = group * a.nq + qt;
@@ -102,7 +74,17 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 ? 1 : 2) v
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
       lse[m] = mine ? a.lse[(bh * MAPS + m) * a.Lq + ic] : INFINITY;
-      del[m] = mine ? a.delta[(bh * MAPS + m) * a.Lq + ic] : 0.f;
+      // D of this lane's query from dO and the saved map result, half a row in each of its two lanes; kept for the other pass
+      const float* o = a.osave + ((bh * a.Lq + ic) * MAPS + m) * a.dv;
+      float d = 0.f;
+#pragma unroll
+      for (int c = 0; c < DV / M::KC; ++c) {
+        const int at = c * M::KC + half * M::NE;
+        if (at < a.dv) d = M::dot(gf[c], o + at, d);
+      }
+      d += __shfl_xor(d, 32);
+      del[m] = m == 0 ? d : -lam * d;
+      if (mine && half == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
 #pragma unroll
       for (int n = 0; n < DQ / 32; ++n) acc[m][n] = zero16();
     }
@@ -112,27 +94,42 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 ? 1 : 2) v
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
     int done = line_begin;                                       // line places that are written
 
-    for (int t = 0; t < tiles; ++t) {
+    St next;
+    auto fetch = [&](int t) {
+      const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
+      next.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.ks[2], a.d, vp + (int64_t)j0 * a.vs[1], a.vs[1], a.dv, valid,
+                line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
+    };
+    auto put = [&](int t, char* to) {
       const int j0 = t * KEYS, valid = min(len - j0, KEYS);
-      const int kfirst = grid_code(j0, a.gw), base = kfirst - code_last + a.line_off;
-      const int wlen = grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1;
+      int* codes = reinterpret_cast<int*>(to + St::TILES);
+      next.store(reinterpret_cast<T*>(to), reinterpret_cast<float*>(codes + KEYS));
+      if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - grid_code(j0, a.gw);
+    };
+    __syncthreads();                                             // the image before this one is done with the buffers
+    if (tiles) {
+      fetch(0);
+      put(0, smem);
+    }
+    for (int t = 0; t < tiles; ++t) {
+      const int base = grid_code(t * KEYS, a.gw) - code_last + a.line_off, valid = min(len - t * KEYS, KEYS);
+      char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
       __syncthreads();
-      if (BIAS) {                                                // a place's thread is the same for every image
+      if (NBUF == 2 && t + 1 < tiles) fetch(t + 1);
+      if (BIAS && done < base) {                                 // a place's thread is the same for every image
         for (int w = done + ((int)threadIdx.x - done & 255); w < base; w += 64 * WAVES) {
           const double s = take_place<ROW4>(ring, (unsigned)w % size, size);
           line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
         }
         done = base;
+        __syncthreads();
       }
       const unsigned ring_base = (unsigned)base % size;
-#pragma unroll
-      for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Ks + m * KEYS * SQ, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
-      stage_rows<T, DV, KEYS>(Vs, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
-      if (threadIdx.x < KEYS) kc[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
-      for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
-      __syncthreads();
-      if (!busy) continue;
-
+      const T* Ks = reinterpret_cast<const T*>(at);
+      const T* Vs = Ks + MAPS * KEYS * SQ;
+      const int* kc = reinterpret_cast<const int*>(at + St::TILES);
+      const float* win = reinterpret_cast<const float*>(kc + KEYS);
+      if (busy)
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
         if (sub * 32 >= valid) break;
@@ -192,6 +189,13 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 ? 1 : 2) v
             for (int n = 0; n < DQ / 32; ++n) acc[m][n] = M::mma(M::load_t(Ks + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, acc[m][n]);
           }
       }
+      if (t + 1 < tiles) {
+        if (NBUF == 1) {
+          __syncthreads();
+          fetch(t + 1);
+        }
+        put(t + 1, NBUF == 2 && !(t & 1) ? smem + buffer : smem);
+      }
     }
 
     if (BIAS) {
@@ -232,14 +236,13 @@ template <typename T, int DQ, int DV, int MAPS, bool ROW4>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
+  using St = Stage<T, DQ, DV, MAPS>;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NBUF = buffers<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* Qs = reinterpret_cast<T*>(smem);
-  T* Gs = Qs + MAPS * KEYS * SQ;
-  int* qc = reinterpret_cast<int*>(Gs + KEYS * SV);
-  float* rows = reinterpret_cast<float*>(qc + KEYS);             // [2][MAPS][KEYS]: log-sums, D
-  float* win = rows + 2 * MAPS * KEYS + 4;                       // four zeros in front: behind the last query a run of four reaches there
-  if (threadIdx.x < 4) win[(int)threadIdx.x - 4] = 0.f;
+  // tiles, codes, [2][MAPS][KEYS] log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
+  const size_t buffer = St::TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
+  if (threadIdx.x < 4 * NBUF)
+    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + St::TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
@@ -267,28 +270,41 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(MAPS * h) * a.qs[2];
   const T* gp = static_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * a.dv;
   const int tiles = k0 < len ? (a.Lq + KEYS - 1) / KEYS : 0;
+  St next;
+  float next_row = 0.f;
+  auto fetch = [&](int t) {
+    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS), code_last = grid_code(a.q_start + i0 + valid - 1, a.gw);
+    next.load(qp + (int64_t)i0 * a.qs[1], a.qs[1], a.qs[2], a.d, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, a.dv, valid,
+              line + code_first - code_last + a.line_off, code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1);
+    const int which = threadIdx.x / KEYS, i = threadIdx.x % KEYS;             // log-sums of the maps, then D
+    if (which < 2 * MAPS) {
+      const float* from = which < MAPS ? a.lse : a.delta;
+      next_row = i < valid ? from[((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + i] : which < MAPS ? INFINITY : 0.f;   // behind the last query: P = 0
+    }
+  };
+  auto put = [&](int t, char* to) {
+    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS), code_last = grid_code(a.q_start + i0 + valid - 1, a.gw);
+    int* codes = reinterpret_cast<int*>(to + St::TILES);
+    float* rows = reinterpret_cast<float*>(codes + KEYS);
+    next.store(reinterpret_cast<T*>(to), rows + 2 * MAPS * KEYS + 4);
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = code_last - grid_code(a.q_start + i0 + min((int)threadIdx.x, valid - 1), a.gw);   // falls along the row
+    if (threadIdx.x < 2 * MAPS * KEYS) rows[threadIdx.x] = next_row;
+  };
+  if (tiles) {
+    fetch(0);
+    put(0, smem);
+  }
   for (int t = 0; t < tiles; ++t) {
-    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS);
-    const int code_last = grid_code(a.q_start + i0 + valid - 1, a.gw), base = code_first - code_last + a.line_off;
-    const int wlen = code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1;
+    char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Qs + m * KEYS * SQ, qp + (int64_t)i0 * a.qs[1] + m * a.qs[2], a.qs[1], valid, a.d);
-    stage_rows<T, DV, KEYS>(Gs, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, valid, a.dv);
-    if (threadIdx.x < KEYS) {
-      const int i = min((int)threadIdx.x, valid - 1);
-      qc[threadIdx.x] = code_last - grid_code(a.q_start + i0 + i, a.gw);   // falls along the row
-    }
-    for (int w = threadIdx.x; w < MAPS * KEYS; w += 64 * WAVES) {
-      const int m = w / KEYS, i = w % KEYS;
-      const int64_t at = ((int64_t)bh * MAPS + m) * a.Lq + i0 + i;
-      rows[w] = i < valid ? a.lse[at] : INFINITY;                // behind the last query: probabilities of zero
-      rows[MAPS * KEYS + w] = i < valid ? a.delta[at] : 0.f;
-    }
-    for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
-    __syncthreads();
-    if (!busy) continue;
-
+    if (NBUF == 2 && t + 1 < tiles) fetch(t + 1);
+    const T* Qs = reinterpret_cast<const T*>(at);
+    const T* Gs = Qs + MAPS * KEYS * SQ;
+    const int* qc = reinterpret_cast<const int*>(at + St::TILES);
+    const float* rows = reinterpret_cast<const float*>(qc + KEYS);
+    const float* win = rows + 2 * MAPS * KEYS + 4;
+    const int valid = min(a.Lq - t * KEYS, KEYS);
+    if (busy)
 #pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
       if (sub * 32 >= valid) break;
@@ -331,6 +347,13 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
           for (int n = 0; n < DQ / 32; ++n) dk[m][n] = M::mma(M::load_t(Qs + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, dk[m][n]);
         }
       }
+    }
+    if (t + 1 < tiles) {
+      if (NBUF == 1) {
+        __syncthreads();
+        fetch(t + 1);
+      }
+      put(t + 1, NBUF == 2 && !(t & 1) ? smem + buffer : smem);
     }
   }
   if (j >= a.Lk) return;
@@ -442,31 +465,29 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   return l;
 }
 
-template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, int window, hipStream_t st) {
+template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
   auto kern = a.row4 ? attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, true> : attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, false>;
-  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 256 +
-                      (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8 + (size_t)round64(window + 4) * 4;
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + KEYS * 4 + (size_t)a.window * 4) +
+                      (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_q_kernel");
 }
 
-template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, int window, float* delta, hipStream_t st) {
-  hipLaunchKernelGGL((attn_delta_kernel<T, MAPS>), dim3((unsigned)cdiv((int64_t)a.B * a.H * a.Lq, 16)), dim3(256), 0, st, a, delta);
-  if (int rc = check_launch("attn_delta_kernel")) return rc;
-  if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, window, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, window, st)) return rc;
+template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, hipStream_t st) {
+  if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, st)) return rc;
   auto kern = a.row4 && a.q_start % 4 == 0 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, true> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, false>;
-  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + 2 * MAPS * KEYS * 4 + (size_t)round64(window + 4) * 4;
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_kv_kernel");
 }
 
-template <typename T> static int dispatch_bwd(const AttnArgs& a, int maps, int window, float* delta, hipStream_t st) {
-  if (maps == 2) return a.d <= 32 ? launch_bwd<T, 32, 64, 2>(a, window, delta, st) : launch_bwd<T, 64, 128, 2>(a, window, delta, st);
-  if (a.d <= 32) return launch_bwd<T, 32, 32, 1>(a, window, delta, st);
-  if (a.d <= 64) return launch_bwd<T, 64, 64, 1>(a, window, delta, st);
-  return launch_bwd<T, 128, 128, 1>(a, window, delta, st);
+template <typename T> static int dispatch_bwd(const AttnArgs& a, int maps, hipStream_t st) {
+  if (maps == 2) return a.d <= 32 ? launch_bwd<T, 32, 64, 2>(a, st) : launch_bwd<T, 64, 128, 2>(a, st);
+  if (a.d <= 32) return launch_bwd<T, 32, 32, 1>(a, st);
+  if (a.d <= 64) return launch_bwd<T, 64, 64, 1>(a, st);
+  return launch_bwd<T, 128, 128, 1>(a, st);
 }
 
 }  // namespace im2im
@@ -502,16 +523,14 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   const BwdLayout l = bwd_layout(a, p->maps, table);
   IM2IM_REQUIRE(ws && ws_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
   char* w = static_cast<char*>(ws);
-  float* delta = reinterpret_cast<float*>(w + l.delta);
-  a.dout = g->dout; a.lse = const_cast<float*>(g->lse); a.osave = const_cast<float*>(g->map_out); a.delta = delta;
+  a.dout = g->dout; a.lse = const_cast<float*>(g->lse); a.osave = const_cast<float*>(g->map_out); a.delta = reinterpret_cast<float*>(w + l.delta);
   a.dq = g->dq; a.dk = g->dk; a.dvv = g->dv;
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
   a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
-  const int window = window_floats(p->gh, p->gw);
-  a.ring = round64(window);
+  a.ring = round64(window_floats(p->gh, p->gw));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, window, delta, st) : dispatch_bwd<float>(a, p->maps, window, delta, st)) return rc;
+  if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, st) : dispatch_bwd<float>(a, p->maps, st)) return rc;
   double* line = reinterpret_cast<double*>(w + l.line);
   if (table) {
     hipLaunchKernelGGL(attn_line_sum_kernel, dim3((unsigned)cdiv(a.line_len, 64), (unsigned)a.H), dim3(256), 0, st, a, line);

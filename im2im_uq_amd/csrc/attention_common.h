@@ -24,6 +24,7 @@ struct AttnArgs {
   const int32_t* lengths;             // [B] or null
   const float* lam;                   // [H] (two maps)
   int B, Lq, Lk, H, d, dv, gw, line_len, line_off, q_start, nq, nk;
+  int window;                         // floats of LDS for the window of `line` that a tile reaches
   int row4;                           // any four tokens from a multiple of four on lie side by side in the grid
   float scale;                        // of the scores
   // forward
@@ -35,7 +36,7 @@ struct AttnArgs {
   int splits, tiles_per_split;
   // backward
   const void* dout;                   // [B][Lq][H][dv]
-  const float* delta;                 // [B*H][MAPS][Lq]
+  float* delta;                       // [B*H][MAPS][Lq]: D
   void *dq, *dk, *dvv;
   int64_t dqs[3], dks[3], dvs[3];
   float* line_part;                   // [nq * groups][H][line_len] or null
@@ -69,6 +70,15 @@ template <> struct Mma<bf16_t> {
     for (int e = 0; e < 8; ++e) r[e] = (__bf16)(s[8 * t + e] - (float)h[e]);
     return __builtin_bit_cast(short8, r);
   }
+  static __device__ __forceinline__ float dot(Frag f, const float* x, float acc) {
+    const bf16x8 v = as_bf16x8(f);
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(x), hi = *reinterpret_cast<const f32x4*>(x + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = fmaf((float)v[e], lo[e], acc);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = fmaf((float)v[4 + e], hi[e], acc);
+    return acc;
+  }
   // left operand taken transposed from an LDS tile [rows][stride]: lane = column col0 + l % 32, reduction = rows row0 + row(NE t + e)
   static __device__ __forceinline__ Frag load_t(const bf16_t* tile, int stride, int row0, int t, int col0) {
     const int lane = threadIdx.x & 63, q = lane & 15;
@@ -89,6 +99,12 @@ template <> struct Mma<float> {
   }
   static __device__ __forceinline__ Frag pack(const f32x16& s, int t) { return f32x4{s[4 * t], s[4 * t + 1], s[4 * t + 2], s[4 * t + 3]}; }
   static __device__ __forceinline__ Frag pack_rest(const f32x16&, Frag, int) { return zero(); }
+  static __device__ __forceinline__ float dot(Frag f, const float* x, float acc) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = fmaf(f[e], v[e], acc);
+    return acc;
+  }
   static __device__ __forceinline__ Frag load_t(const float* tile, int stride, int row0, int t, int col0) {
     const int lane = threadIdx.x & 63;
     const float* p = tile + (size_t)(row0 + 8 * t + 4 * (lane >> 5)) * stride + col0 + (lane & 31);
@@ -114,21 +130,68 @@ template <typename T, int D> __device__ __forceinline__ void load_row_frags(type
   }
 }
 
-// rows [0, NR) of a tile into LDS by the whole workgroup; rows from `valid` on and elements from d on are zeros (masked rows may hold
-// anything, infinities and NaN too: a zero probability does not silence them in a product, a zero operand does)
-template <typename T, int D, int NR> __device__ __forceinline__ void stage_rows(T* dst, const T* src, int64_t stride, int valid, int d) {
-  constexpr int V = 16 / (int)sizeof(T), PR = D / V, S = padded<T>(D);
+// rows [0, NR) of a tile on their way into LDS by the whole workgroup: in registers between load() and store(), so that the next tile's
+// loads run behind this tile's work.  Rows from `valid` on and elements from d on are zeros (masked rows may hold anything, infinities
+// and NaN too: a zero probability does not silence them in a product, a zero operand does).
+template <typename T, int D, int NR> struct TileRegs {
+  static constexpr int V = 16 / (int)sizeof(T), PR = D / V, S = padded<T>(D), N = NR * PR / (64 * WAVES);
+  static_assert(NR * PR % (64 * WAVES) == 0, "whole rounds of the workgroup");
+  u32x4 x[N];
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int valid, int d) {
 #pragma unroll
-  for (int i0 = 0; i0 < NR * PR; i0 += 64 * WAVES) {
-    const int i = i0 + threadIdx.x;
-    if (NR * PR % (64 * WAVES) == 0 || i < NR * PR) {
-      const int r = i / PR, c = (i % PR) * V;
-      u32x4 x = {0, 0, 0, 0};
-      if (r < valid && c < d) x = *reinterpret_cast<const u32x4*>(src + r * stride + c);
-      *reinterpret_cast<u32x4*>(dst + r * S + c) = x;
+    for (int n = 0; n < N; ++n) {
+      const int i = n * 64 * WAVES + threadIdx.x, r = i / PR, c = (i % PR) * V;
+      x[n] = u32x4{0, 0, 0, 0};
+      if (r < valid && c < d) x[n] = *reinterpret_cast<const u32x4*>(src + r * stride + c);
     }
   }
-}
+  __device__ __forceinline__ void store(T* dst) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = n * 64 * WAVES + threadIdx.x;
+      *reinterpret_cast<u32x4*>(dst + (i / PR) * S + (i % PR) * V) = x[n];
+    }
+  }
+};
+
+// LDS buffers of tiles: two where a row of both fits 512 bytes (64 KiB of tiles), one for the widest heads in 32 bits
+template <typename T> __host__ __device__ constexpr int buffers(int elements) { return elements * (int)sizeof(T) <= 512 ? 2 : 1; }
+
+// The two tiles of an iteration (KEYS rows of MAPS x DQ and of DV elements), the codes of their rows and the window of `line` that they reach.
+// With two of these in LDS an iteration has one barrier.
+template <typename T, int DQ, int DV, int MAPS> struct Stage {
+  static constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
+  static constexpr size_t TILES = (size_t)KEYS * (MAPS * SQ + SV) * sizeof(T);
+  static constexpr int WIN_REGS = 2;
+  TileRegs<T, DQ, KEYS> a[MAPS];
+  TileRegs<T, DV, KEYS> b;
+  float win[WIN_REGS];
+  const float* line;
+  int wlen;
+  __device__ __forceinline__ void load(const T* pa, int64_t sa, int64_t map_a, int d, const T* pb, int64_t sb, int dv, int valid, const float* line_, int wlen_) {
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) a[m].load(pa + m * map_a, sa, valid, d);
+    b.load(pb, sb, valid, dv);
+    line = line_;
+    wlen = wlen_;
+#pragma unroll
+    for (int n = 0; n < WIN_REGS; ++n) {
+      const int w = n * 64 * WAVES + threadIdx.x;
+      win[n] = w < wlen ? line[w] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(T* tiles, float* window) const {
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) a[m].store(tiles + m * KEYS * SQ);
+    b.store(tiles + MAPS * KEYS * SQ);
+#pragma unroll
+    for (int n = 0; n < WIN_REGS; ++n) {
+      const int w = n * 64 * WAVES + threadIdx.x;
+      if (w < wlen) window[w] = win[n];
+    }
+    for (int w = WIN_REGS * 64 * WAVES + threadIdx.x; w < wlen; w += 64 * WAVES) window[w] = line[w];      // grids over 120 wide
+  }
+};
 
 // the bias of a lane's 16 scores: places codes[row] + off of the window.  ROW4: four rows' codes are consecutive (rising or falling), one place
 // serves them; behind the last valid row that may reach three places over the window's end, values that the callers mask.

@@ -49,15 +49,13 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 constexpr float GROW = 8.f;
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4>
-__global__ __launch_bounds__(64 * WAVES, MAPS * DV >= 256 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NB = DV / 32;
+  using St = Stage<T, DQ, DV, MAPS>;
+  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  T* Ks = reinterpret_cast<T*>(smem);
-  T* Vs = Ks + MAPS * KEYS * SQ;
-  int* kc = reinterpret_cast<int*>(Vs + KEYS * SV);
-  float* win = reinterpret_cast<float*>(kc + KEYS);
+  const size_t buffer = St::TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.splits, item = lin / a.splits;
   const int qt = item % a.nq, bh = item / a.nq, h = bh % a.H, b = bh / a.H;
@@ -91,19 +89,32 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV >= 256 ? 1 : 2) void attn_fwd
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
   const float* line = a.line + (int64_t)h * a.line_len;
 
-  for (int t = t0; t < t1; ++t) {
+  St next;
+  auto fetch = [&](int t) {
+    const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
+    next.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.ks[2], a.d, vp + (int64_t)j0 * a.vs[1], a.vs[1], a.dv, valid, line + kfirst - code_last + a.line_off,
+              grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
+  };
+  auto put = [&](int t, char* to) {
     const int j0 = t * KEYS, valid = min(len - j0, KEYS);
-    const int kfirst = grid_code(j0, a.gw), base = kfirst - code_last + a.line_off;
-    const int wlen = grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1;
+    int* codes = reinterpret_cast<int*>(to + St::TILES);
+    next.store(reinterpret_cast<T*>(to), reinterpret_cast<float*>(codes + KEYS));
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - grid_code(j0, a.gw);
+  };
+  if (t0 < t1) {
+    fetch(t0);
+    put(t0, smem);
+  }
+  for (int t = t0; t < t1; ++t) {
+    char* at = smem + (NBUF == 2 && ((t - t0) & 1) ? buffer : 0);
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) stage_rows<T, DQ, KEYS>(Ks + m * KEYS * SQ, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
-    stage_rows<T, DV, KEYS>(Vs, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
-    if (threadIdx.x < KEYS) kc[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
-    for (int w = threadIdx.x; w < wlen; w += 64 * WAVES) win[w] = line[base + w];
-    __syncthreads();
-    if (!busy) continue;
-
+    if (NBUF == 2 && t + 1 < t1) fetch(t + 1);
+    const T* Ks = reinterpret_cast<const T*>(at);
+    const T* Vs = Ks + MAPS * KEYS * SQ;
+    const int* kc = reinterpret_cast<const int*>(at + St::TILES);
+    const float* win = reinterpret_cast<const float*>(kc + KEYS);
+    const int valid = min(len - t * KEYS, KEYS);
+    if (busy)
 #pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
       if (sub * 32 >= valid) break;
@@ -166,6 +177,13 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV >= 256 ? 1 : 2) void attn_fwd
           }
         }
       }
+    }
+    if (t + 1 < t1) {
+      if (NBUF == 1) {
+        __syncthreads();
+        fetch(t + 1);
+      }
+      put(t + 1, NBUF == 2 && !((t - t0) & 1) ? smem + buffer : smem);
     }
   }
 
@@ -352,6 +370,7 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   a->nq = (int)cdiv(p->Lq, ROWS);
   a->nk = (int)cdiv(p->Lk, ROWS);
   a->scale = p->scale;
+  a->window = round64(window_floats(p->gh, p->gw) + 4);            // a run of four may reach three over the end
   IM2IM_REQUIRE((int64_t)p->B * p->H * p->Lq < (1ll << 31) && (int64_t)p->B * p->H * a->nk < (1ll << 31) / 64);
   return IM2IM_OK;
 }
@@ -366,9 +385,9 @@ static int key_splits(const AttnArgs& a) {
   return (int)cdiv(tiles, cdiv(tiles, n));
 }
 
-template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, int window, hipStream_t st) {
+template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
   auto kern = a.row4 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, true> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, false>;
-  const size_t smem = (size_t)KEYS * (MAPS * padded<T>(DQ) + padded<T>(DV)) * sizeof(T) + KEYS * 4 + (size_t)round64(window + 4) * 4;
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + KEYS * 4 + (size_t)a.window * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nq * a.splits)), dim3(64 * WAVES), smem, st, a);
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
@@ -381,11 +400,11 @@ template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd
   return IM2IM_OK;
 }
 
-template <typename T, bool SAVE> static int dispatch_fwd(const AttnArgs& a, int maps, int window, hipStream_t st) {
-  if (maps == 2) return a.d <= 32 ? launch_fwd<T, 32, 64, 2, SAVE>(a, window, st) : launch_fwd<T, 64, 128, 2, SAVE>(a, window, st);
-  if (a.d <= 32) return launch_fwd<T, 32, 32, 1, SAVE>(a, window, st);
-  if (a.d <= 64) return launch_fwd<T, 64, 64, 1, SAVE>(a, window, st);
-  return launch_fwd<T, 128, 128, 1, SAVE>(a, window, st);
+template <typename T, bool SAVE> static int dispatch_fwd(const AttnArgs& a, int maps, hipStream_t st) {
+  if (maps == 2) return a.d <= 32 ? launch_fwd<T, 32, 64, 2, SAVE>(a, st) : launch_fwd<T, 64, 128, 2, SAVE>(a, st);
+  if (a.d <= 32) return launch_fwd<T, 32, 32, 1, SAVE>(a, st);
+  if (a.d <= 64) return launch_fwd<T, 64, 64, 1, SAVE>(a, st);
+  return launch_fwd<T, 128, 128, 1, SAVE>(a, st);
 }
 
 }  // namespace im2im
@@ -432,8 +451,7 @@ extern "C" int im2im_attention_fwd(const im2im_attention_desc* p, void* out, flo
     a.part = static_cast<float*>(ws);
     a.part_ml = a.part + rows * a.dv;
   }
-  const int window = window_floats(p->gh, p->gw);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p->dtype == IM2IM_BF16) return lse ? dispatch_fwd<bf16_t, true>(a, p->maps, window, st) : dispatch_fwd<bf16_t, false>(a, p->maps, window, st);
-  return lse ? dispatch_fwd<float, true>(a, p->maps, window, st) : dispatch_fwd<float, false>(a, p->maps, window, st);
+  if (p->dtype == IM2IM_BF16) return lse ? dispatch_fwd<bf16_t, true>(a, p->maps, st) : dispatch_fwd<bf16_t, false>(a, p->maps, st);
+  return lse ? dispatch_fwd<float, true>(a, p->maps, st) : dispatch_fwd<float, false>(a, p->maps, st);
 }
