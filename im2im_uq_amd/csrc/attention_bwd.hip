@@ -33,10 +33,10 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  using St = Stage<T, DQ, DV, MAPS>;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const size_t buffer = St::TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
+  const size_t buffer = TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
   double* ring = reinterpret_cast<double*>(smem + NBUF * buffer);          // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
   __shared__ float red[WAVES];
 
@@ -94,40 +94,34 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
     int done = line_begin;                                       // line places that are written
 
-    St next;
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t, char* to) {
       const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
-      next.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.ks[2], a.d, vp + (int64_t)j0 * a.vs[1], a.vs[1], a.dv, valid,
-                line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
-    };
-    auto put = [&](int t, char* to) {
-      const int j0 = t * KEYS, valid = min(len - j0, KEYS);
-      int* codes = reinterpret_cast<int*>(to + St::TILES);
-      next.store(reinterpret_cast<T*>(to), reinterpret_cast<float*>(codes + KEYS));
-      if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - grid_code(j0, a.gw);
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * QT, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
+      fetch_tile<T, DV>(to + MAPS * QT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+      int* codes = reinterpret_cast<int*>(to + TILES);
+      fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
+      if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
     };
     __syncthreads();                                             // the image before this one is done with the buffers
-    if (tiles) {
-      fetch(0);
-      put(0, smem);
-    }
+    if (tiles) fetch(0, smem);
     for (int t = 0; t < tiles; ++t) {
       const int base = grid_code(t * KEYS, a.gw) - code_last + a.line_off, valid = min(len - t * KEYS, KEYS);
       char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
+      lds_loads_done();
       __syncthreads();
-      if (NBUF == 2 && t + 1 < tiles) fetch(t + 1);
       if (BIAS && done < base) {                                 // a place's thread is the same for every image
         for (int w = done + ((int)threadIdx.x - done & 255); w < base; w += 64 * WAVES) {
           const double s = take_place<ROW4>(ring, (unsigned)w % size, size);
           line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
         }
         done = base;
-        __syncthreads();
+        if (!a.ring_wide) __syncthreads();                       // else the places that this tile adds to are others
       }
+      if (NBUF == 2 && t + 1 < tiles) fetch(t + 1, t & 1 ? smem : smem + buffer);
       const unsigned ring_base = (unsigned)base % size;
-      const T* Ks = reinterpret_cast<const T*>(at);
-      const T* Vs = Ks + MAPS * KEYS * SQ;
-      const int* kc = reinterpret_cast<const int*>(at + St::TILES);
+      const char *Ks = at, *Vs = at + MAPS * QT;
+      const int* kc = reinterpret_cast<const int*>(at + TILES);
       const float* win = reinterpret_cast<const float*>(kc + KEYS);
       if (busy)
 #pragma unroll 1
@@ -142,11 +136,11 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
           s[m] = zero16();
 #pragma unroll
           for (int c = 0; c < DQ / M::KC; ++c)
-            s[m] = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], s[m]);
+            s[m] = M::mma(tile_frag<T, DQ>(Ks + m * QT, sub * 32, c), qf[m][c], s[m]);
         }
 #pragma unroll
         for (int c = 0; c < DV / M::KC; ++c)
-          dp = M::mma(load_frag<T>(Vs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), gf[c], dp);
+          dp = M::mma(tile_frag<T, DV>(Vs, sub * 32, c), gf[c], dp);
 #pragma unroll
         for (int m = 0; m < MAPS; ++m)
 #pragma unroll
@@ -186,15 +180,12 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
           for (int m = 0; m < MAPS; ++m) {
             const Frag df = M::pack(s[m], ks);
 #pragma unroll
-            for (int n = 0; n < DQ / 32; ++n) acc[m][n] = M::mma(M::load_t(Ks + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, acc[m][n]);
+            for (int n = 0; n < DQ / 32; ++n) acc[m][n] = M::mma(M::template load_t<DQ>(Ks + m * QT, sub * 32, ks, n), df, acc[m][n]);
           }
       }
-      if (t + 1 < tiles) {
-        if (NBUF == 1) {
-          __syncthreads();
-          fetch(t + 1);
-        }
-        put(t + 1, NBUF == 2 && !(t & 1) ? smem + buffer : smem);
+      if (NBUF == 1 && t + 1 < tiles) {
+        __syncthreads();
+        fetch(t + 1, smem);
       }
     }
 
@@ -236,13 +227,13 @@ template <typename T, int DQ, int DV, int MAPS, bool ROW4>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  using St = Stage<T, DQ, DV, MAPS>;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // tiles, codes, [2][MAPS][KEYS] log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
-  const size_t buffer = St::TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
+  const size_t buffer = TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
   if (threadIdx.x < 4 * NBUF)
-    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + St::TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
+    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
@@ -270,37 +261,29 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(MAPS * h) * a.qs[2];
   const T* gp = static_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * a.dv;
   const int tiles = k0 < len ? (a.Lq + KEYS - 1) / KEYS : 0;
-  St next;
-  float next_row = 0.f;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, char* to) {
     const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS), code_last = grid_code(a.q_start + i0 + valid - 1, a.gw);
-    next.load(qp + (int64_t)i0 * a.qs[1], a.qs[1], a.qs[2], a.d, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, a.dv, valid,
-              line + code_first - code_last + a.line_off, code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1);
-    const int which = threadIdx.x / KEYS, i = threadIdx.x % KEYS;             // log-sums of the maps, then D
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * QT, qp + (int64_t)i0 * a.qs[1] + m * a.qs[2], a.qs[1], valid, a.d);
+    fetch_tile<T, DV>(to + MAPS * QT, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, valid, a.dv);
+    int* codes = reinterpret_cast<int*>(to + TILES);
+    float* rows = reinterpret_cast<float*>(codes + KEYS);
+    const int which = wave_index();                              // a wave fetches log-sums (infinite behind the last query: P = 0) or D of a map
     if (which < 2 * MAPS) {
       const float* from = which < MAPS ? a.lse : a.delta;
-      next_row = i < valid ? from[((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + i] : which < MAPS ? INFINITY : 0.f;   // behind the last query: P = 0
+      load4_to_lds(lane < valid ? from + ((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + lane : attn_fill + (which < MAPS ? 4 : 0), rows + which * KEYS);
     }
-  };
-  auto put = [&](int t, char* to) {
-    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS), code_last = grid_code(a.q_start + i0 + valid - 1, a.gw);
-    int* codes = reinterpret_cast<int*>(to + St::TILES);
-    float* rows = reinterpret_cast<float*>(codes + KEYS);
-    next.store(reinterpret_cast<T*>(to), rows + 2 * MAPS * KEYS + 4);
+    fetch_window(rows + 2 * MAPS * KEYS + 4, line + code_first - code_last + a.line_off, code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1);
     if (threadIdx.x < KEYS) codes[threadIdx.x] = code_last - grid_code(a.q_start + i0 + min((int)threadIdx.x, valid - 1), a.gw);   // falls along the row
-    if (threadIdx.x < 2 * MAPS * KEYS) rows[threadIdx.x] = next_row;
   };
-  if (tiles) {
-    fetch(0);
-    put(0, smem);
-  }
+  if (tiles) fetch(0, smem);
   for (int t = 0; t < tiles; ++t) {
     char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
+    lds_loads_done();
     __syncthreads();
-    if (NBUF == 2 && t + 1 < tiles) fetch(t + 1);
-    const T* Qs = reinterpret_cast<const T*>(at);
-    const T* Gs = Qs + MAPS * KEYS * SQ;
-    const int* qc = reinterpret_cast<const int*>(at + St::TILES);
+    if (NBUF == 2 && t + 1 < tiles) fetch(t + 1, t & 1 ? smem : smem + buffer);
+    const char *Qs = at, *Gs = at + MAPS * QT;
+    const int* qc = reinterpret_cast<const int*>(at + TILES);
     const float* rows = reinterpret_cast<const float*>(qc + KEYS);
     const float* win = rows + 2 * MAPS * KEYS + 4;
     const int valid = min(a.Lq - t * KEYS, KEYS);
@@ -316,11 +299,11 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
         s[m] = zero16();
 #pragma unroll
         for (int c = 0; c < DQ / M::KC; ++c)
-          s[m] = M::mma(load_frag<T>(Qs + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), kf[m][c], s[m]);
+          s[m] = M::mma(tile_frag<T, DQ>(Qs + m * QT, sub * 32, c), kf[m][c], s[m]);
       }
 #pragma unroll
       for (int c = 0; c < DV / M::KC; ++c)
-        dp = M::mma(load_frag<T>(Gs + (sub * 32 + (lane & 31)) * SV + c * M::KC + half * M::NE), vf[c], dp);
+        dp = M::mma(tile_frag<T, DV>(Gs, sub * 32, c), vf[c], dp);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -339,21 +322,18 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
       for (int ks = 0; ks < 32 / M::KC; ++ks) {
         const Frag pf = M::pack(mix, ks);
 #pragma unroll
-        for (int n = 0; n < DV / 32; ++n) dv[n] = M::mma(M::load_t(Gs, SV, sub * 32, ks, n * 32), pf, dv[n]);
+        for (int n = 0; n < DV / 32; ++n) dv[n] = M::mma(M::template load_t<DV>(Gs, sub * 32, ks, n), pf, dv[n]);
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
           const Frag df = M::pack(s[m], ks);
 #pragma unroll
-          for (int n = 0; n < DQ / 32; ++n) dk[m][n] = M::mma(M::load_t(Qs + m * KEYS * SQ, SQ, sub * 32, ks, n * 32), df, dk[m][n]);
+          for (int n = 0; n < DQ / 32; ++n) dk[m][n] = M::mma(M::template load_t<DQ>(Qs + m * QT, sub * 32, ks, n), df, dk[m][n]);
         }
       }
     }
-    if (t + 1 < tiles) {
-      if (NBUF == 1) {
-        __syncthreads();
-        fetch(t + 1);
-      }
-      put(t + 1, NBUF == 2 && !(t & 1) ? smem + buffer : smem);
+    if (NBUF == 1 && t + 1 < tiles) {
+      __syncthreads();
+      fetch(t + 1, smem);
     }
   }
   if (j >= a.Lk) return;
@@ -446,10 +426,12 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 
 // -------------------------------------------------------------------------------------------------------------------- host
 
-// images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, so their number (about 1024)
-// bounds that memory
+// images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, in at most 256 MiB where one image a
+// workgroup would take more (several add to their line in memory, a read and a wait a tile)
 static void set_groups(AttnArgs* a) {
-  a->group_images = (int)std::max<int64_t>(1, std::min<int64_t>(a->B, (int64_t)a->B * a->H * a->nq / 1024));
+  const int64_t line = (int64_t)a->H * a->nq * a->line_len * 4;
+  a->groups = (int)std::max<int64_t>(1, std::min<int64_t>(a->B, (256ll << 20) / line));
+  a->group_images = (int)cdiv(a->B, a->groups);
   a->groups = (int)cdiv(a->B, a->group_images);
 }
 
@@ -467,7 +449,7 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
 
 template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
   auto kern = a.row4 ? attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, true> : attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, false>;
-  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + KEYS * 4 + (size_t)a.window * 4) +
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4) +
                       (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq)), dim3(64 * WAVES), smem, st, a);
@@ -477,7 +459,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd
 template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, hipStream_t st) {
   if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, st)) return rc;
   auto kern = a.row4 && a.q_start % 4 == 0 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, true> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, false>;
-  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_kv_kernel");
@@ -528,7 +510,11 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
   a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
-  a.ring = round64(window_floats(p->gh, p->gw));
+  // a ring of the window and one tile's advance: a tile's places are then none of those that are being written, and one barrier a tile will do.
+  // Where LDS does not hold that (grids over 278 wide), the window alone, and a second barrier.
+  a.ring = round64(window_floats(p->gh, p->gw) + code_span(KEYS + 1, p->gh, p->gw));
+  a.ring_wide = a.ring <= 1088;
+  if (!a.ring_wide) a.ring = round64(window_floats(p->gh, p->gw));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, st) : dispatch_bwd<float>(a, p->maps, st)) return rc;
   double* line = reinterpret_cast<double*>(w + l.line);

@@ -41,12 +41,19 @@ struct AttnArgs {
   int64_t dqs[3], dks[3], dvs[3];
   float* line_part;                   // [nq * groups][H][line_len] or null
   float* dlam_part;                   // [nq * groups][H]
-  int groups, group_images, ring;     // ring: places in one copy of the LDS accumulator
+  int groups, group_images, ring, ring_wide;   // ring: places in one copy of the LDS accumulator
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int KEYS = 64;              // keys (queries in the key-gradient kernel) of one LDS tile
 constexpr int WAVES = 4, ROWS = 32 * WAVES;   // queries (keys) of a workgroup: 32 columns for each wave
+
+// Where 16-byte piece `slot` of row r (0..15, and on in steps of 16 rows) of an LDS tile with BYTES a row lies: rows are dense, their pieces
+// permuted so that both ways of reading a tile meet all 64 banks: 16 rows' piece of the same place, and 4 rows' 64-byte stretch (transposed).
+template <int BYTES> __device__ __forceinline__ int place(int r, int slot) {
+  const int s = BYTES == 64 ? (r >> 2) & 3 : BYTES == 128 ? (r & 2) << 1 | (r & 4) >> 1 | (r & 8) >> 3 : (r & 3) << 2 | (r >> 2 & 3);
+  return r * BYTES + ((slot ^ s) << 4);
+}
 
 template <typename T> struct Mma;
 template <> struct Mma<bf16_t> {
@@ -79,12 +86,12 @@ template <> struct Mma<bf16_t> {
     for (int e = 0; e < 4; ++e) acc = fmaf((float)v[4 + e], hi[e], acc);
     return acc;
   }
-  // left operand taken transposed from an LDS tile [rows][stride]: lane = column col0 + l % 32, reduction = rows row0 + row(NE t + e)
-  static __device__ __forceinline__ Frag load_t(const bf16_t* tile, int stride, int row0, int t, int col0) {
-    const int lane = threadIdx.x & 63, q = lane & 15;
-    const bf16_t* p = tile + (size_t)(row0 + 16 * t + 4 * (lane >> 5) + (q >> 2)) * stride + col0 + 16 * ((lane >> 4) & 1) + 4 * (q & 3);
-    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)reinterpret_cast<const char*>(p));
-    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)reinterpret_cast<const char*>(p + 8 * stride));
+  // left operand taken transposed from an LDS tile: lane = column 32 n + l % 32, reduction = rows row0 + row(NE t + e)
+  template <int D> static __device__ __forceinline__ Frag load_t(const char* tile, int row0, int t, int n) {
+    const int lane = threadIdx.x & 63, q = lane & 15, r = 4 * (lane >> 5) + (q >> 2), slot = n * 4 + 2 * ((lane >> 4) & 1) + ((q & 3) >> 1);
+    const char* p = tile + (row0 + 16 * t) * (2 * D) + (q & 1) * 8;
+    const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(p + place<D * 2>(r, slot)));
+    const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(lds_char*)(p + place<D * 2>(r + 8, slot)));
     return short8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   }
 };
@@ -105,15 +112,23 @@ template <> struct Mma<float> {
     for (int e = 0; e < 4; ++e) acc = fmaf(f[e], v[e], acc);
     return acc;
   }
-  static __device__ __forceinline__ Frag load_t(const float* tile, int stride, int row0, int t, int col0) {
-    const int lane = threadIdx.x & 63;
-    const float* p = tile + (size_t)(row0 + 8 * t + 4 * (lane >> 5)) * stride + col0 + (lane & 31);
-    return f32x4{p[0], p[stride], p[2 * stride], p[3 * stride]};
+  template <int D> static __device__ __forceinline__ Frag load_t(const char* tile, int row0, int t, int n) {
+    const int lane = threadIdx.x & 63, slot = n * 8 + ((lane & 31) >> 2);
+    const char* p = tile + (row0 + 8 * (t & ~1)) * (4 * D) + (lane & 3) * 4;
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = *reinterpret_cast<const float*>(p + place<D * 4>(8 * (t & 1) + 4 * (lane >> 5) + e, slot));
+    return f;
   }
 };
 
 template <typename T> __device__ __forceinline__ typename Mma<T>::Frag load_frag(const T* p) { return *reinterpret_cast<const typename Mma<T>::Frag*>(p); }
-template <typename T> __host__ __device__ constexpr int padded(int d) { return d + 16 / (int)sizeof(T); }   // LDS row length: 16 rows' 16-byte reads on distinct banks
+// left operand: fragment c of the 32 rows from row0 on
+template <typename T, int D> __device__ __forceinline__ typename Mma<T>::Frag tile_frag(const char* tile, int row0, int c) {
+  const int lane = threadIdx.x & 63;
+  constexpr int BYTES = D * (int)sizeof(T);
+  return *reinterpret_cast<const typename Mma<T>::Frag*>(tile + (row0 + (lane & 16)) * BYTES + place<BYTES>(lane & 15, 2 * c + (lane >> 5)));
+}
 
 __device__ __forceinline__ f32x16 zero16() { return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 __device__ __forceinline__ f32x16 splat16(float v) { return f32x16{v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
@@ -130,68 +145,41 @@ template <typename T, int D> __device__ __forceinline__ void load_row_frags(type
   }
 }
 
-// rows [0, NR) of a tile on their way into LDS by the whole workgroup: in registers between load() and store(), so that the next tile's
-// loads run behind this tile's work.  Rows from `valid` on and elements from d on are zeros (masked rows may hold anything, infinities
-// and NaN too: a zero probability does not silence them in a product, a zero operand does).
-template <typename T, int D, int NR> struct TileRegs {
-  static constexpr int V = 16 / (int)sizeof(T), PR = D / V, S = padded<T>(D), N = NR * PR / (64 * WAVES);
-  static_assert(NR * PR % (64 * WAVES) == 0, "whole rounds of the workgroup");
-  u32x4 x[N];
-  __device__ __forceinline__ void load(const T* src, int64_t stride, int valid, int d) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = n * 64 * WAVES + threadIdx.x, r = i / PR, c = (i % PR) * V;
-      x[n] = u32x4{0, 0, 0, 0};
-      if (r < valid && c < d) x[n] = *reinterpret_cast<const u32x4*>(src + r * stride + c);
-    }
-  }
-  __device__ __forceinline__ void store(T* dst) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = n * 64 * WAVES + threadIdx.x;
-      *reinterpret_cast<u32x4*>(dst + (i / PR) * S + (i % PR) * V) = x[n];
-    }
-  }
-};
+// Loads straight into LDS (global_load_lds): 64 lanes' 16 or 4 bytes, each from its own address, to consecutive places.  What has to be zero (rows
+// behind the last, elements behind a row) or infinite comes from here.  A masked row may hold anything, infinities and NaN too: a zero
+// probability does not silence them in a product, a zero operand does.
+static __device__ const float attn_fill[8] = {0.f, 0.f, 0.f, 0.f, INFINITY, INFINITY, INFINITY, INFINITY};
+__device__ __forceinline__ void load16_to_lds(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+__device__ __forceinline__ void load4_to_lds(const void* from, void* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+// every load of this wave into LDS is there; before the barrier behind which others read it
+__device__ __forceinline__ void lds_loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt 0
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// LDS buffers of tiles: two where a row of both fits 512 bytes (64 KiB of tiles), one for the widest heads in 32 bits
+// KEYS rows of a tile, by the whole workgroup
+template <typename T, int D> __device__ __forceinline__ void fetch_tile(char* to, const T* src, int64_t stride, int valid, int d) {
+  constexpr int BYTES = D * (int)sizeof(T), PR = BYTES / 16, V = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 63, wave = wave_index();
+#pragma unroll
+  for (int n = 0; n < KEYS * PR / (64 * WAVES); ++n) {
+    const int i = (n * WAVES + wave) * 64 + lane, r = i / PR;
+    const int c = ((place<BYTES>(r & 15, i % PR) - (r & 15) * BYTES) >> 4) * V;              // the piece that lies here
+    load16_to_lds(r < valid && c < d ? static_cast<const void*>(src + r * stride + c) : attn_fill, to + (n * WAVES + wave) * 1024);
+  }
+}
+
+// `n` floats of the line, in whole runs of 64 (the window's size in LDS is a multiple of that)
+__device__ __forceinline__ void fetch_window(float* to, const float* line, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int w = wave_index() * 64; w < n; w += 64 * WAVES) load4_to_lds(line + min(w + lane, n - 1), to + w);
+}
+
+// LDS buffers of tiles: two (the next tile's loads run behind this tile's work, one barrier a tile), one for the widest heads in 32 bits
 template <typename T> __host__ __device__ constexpr int buffers(int elements) { return elements * (int)sizeof(T) <= 512 ? 2 : 1; }
-
-// The two tiles of an iteration (KEYS rows of MAPS x DQ and of DV elements), the codes of their rows and the window of `line` that they reach.
-// With two of these in LDS an iteration has one barrier.
-template <typename T, int DQ, int DV, int MAPS> struct Stage {
-  static constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV);
-  static constexpr size_t TILES = (size_t)KEYS * (MAPS * SQ + SV) * sizeof(T);
-  static constexpr int WIN_REGS = 2;
-  TileRegs<T, DQ, KEYS> a[MAPS];
-  TileRegs<T, DV, KEYS> b;
-  float win[WIN_REGS];
-  const float* line;
-  int wlen;
-  __device__ __forceinline__ void load(const T* pa, int64_t sa, int64_t map_a, int d, const T* pb, int64_t sb, int dv, int valid, const float* line_, int wlen_) {
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) a[m].load(pa + m * map_a, sa, valid, d);
-    b.load(pb, sb, valid, dv);
-    line = line_;
-    wlen = wlen_;
-#pragma unroll
-    for (int n = 0; n < WIN_REGS; ++n) {
-      const int w = n * 64 * WAVES + threadIdx.x;
-      win[n] = w < wlen ? line[w] : 0.f;
-    }
-  }
-  __device__ __forceinline__ void store(T* tiles, float* window) const {
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) a[m].store(tiles + m * KEYS * SQ);
-    b.store(tiles + MAPS * KEYS * SQ);
-#pragma unroll
-    for (int n = 0; n < WIN_REGS; ++n) {
-      const int w = n * 64 * WAVES + threadIdx.x;
-      if (w < wlen) window[w] = win[n];
-    }
-    for (int w = WIN_REGS * 64 * WAVES + threadIdx.x; w < wlen; w += 64 * WAVES) window[w] = line[w];      // grids over 120 wide
-  }
-};
+template <typename T> __host__ __device__ constexpr size_t tile_bytes(int elements) { return (size_t)KEYS * elements * sizeof(T); }
 
 // the bias of a lane's 16 scores: places codes[row] + off of the window.  ROW4: four rows' codes are consecutive (rising or falling), one place
 // serves them; behind the last valid row that may reach three places over the window's end, values that the callers mask.

@@ -52,10 +52,10 @@ template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  using St = Stage<T, DQ, DV, MAPS>;
-  constexpr int SQ = padded<T>(DQ), SV = padded<T>(DV), NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr size_t KT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const size_t buffer = St::TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
+  const size_t buffer = TILES + KEYS * 4 + (size_t)a.window * 4;           // tiles, codes, window
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.splits, item = lin / a.splits;
   const int qt = item % a.nq, bh = item / a.nq, h = bh % a.H, b = bh / a.H;
@@ -89,29 +89,23 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
   const float* line = a.line + (int64_t)h * a.line_len;
 
-  St next;
-  auto fetch = [&](int t) {
+  auto fetch = [&](int t, char* to) {
     const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
-    next.load(kp + (int64_t)j0 * a.ks[1], a.ks[1], a.ks[2], a.d, vp + (int64_t)j0 * a.vs[1], a.vs[1], a.dv, valid, line + kfirst - code_last + a.line_off,
-              grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * KT, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
+    fetch_tile<T, DV>(to + MAPS * KT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+    int* codes = reinterpret_cast<int*>(to + TILES);
+    fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
   };
-  auto put = [&](int t, char* to) {
-    const int j0 = t * KEYS, valid = min(len - j0, KEYS);
-    int* codes = reinterpret_cast<int*>(to + St::TILES);
-    next.store(reinterpret_cast<T*>(to), reinterpret_cast<float*>(codes + KEYS));
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - grid_code(j0, a.gw);
-  };
-  if (t0 < t1) {
-    fetch(t0);
-    put(t0, smem);
-  }
+  if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; ++t) {
     char* at = smem + (NBUF == 2 && ((t - t0) & 1) ? buffer : 0);
+    lds_loads_done();
     __syncthreads();
-    if (NBUF == 2 && t + 1 < t1) fetch(t + 1);
-    const T* Ks = reinterpret_cast<const T*>(at);
-    const T* Vs = Ks + MAPS * KEYS * SQ;
-    const int* kc = reinterpret_cast<const int*>(at + St::TILES);
+    if (NBUF == 2 && t + 1 < t1) fetch(t + 1, (t - t0) & 1 ? smem : smem + buffer);
+    const char *Ks = at, *Vs = at + MAPS * KT;
+    const int* kc = reinterpret_cast<const int*>(at + TILES);
     const float* win = reinterpret_cast<const float*>(kc + KEYS);
     const int valid = min(len - t * KEYS, KEYS);
     if (busy)
@@ -126,7 +120,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
         f32x16 acc = zero16();
 #pragma unroll
         for (int c = 0; c < DQ / M::KC; ++c)
-          acc = M::mma(load_frag<T>(Ks + (m * KEYS + sub * 32 + (lane & 31)) * SQ + c * M::KC + half * M::NE), qf[m][c], acc);
+          acc = M::mma(tile_frag<T, DQ>(Ks + m * KT, sub * 32, c), qf[m][c], acc);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[m][r] = fmaf(acc[r], scale2, bias[r]);
       }
@@ -169,7 +163,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const Frag vf = M::load_t(Vs, SV, sub * 32, ks, n * 32);
+          const Frag vf = M::template load_t<DV>(Vs, sub * 32, ks, n);
 #pragma unroll
           for (int m = 0; m < MAPS; ++m) {
             o[m][n] = M::mma(vf, pf[m], o[m][n]);
@@ -178,12 +172,9 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
         }
       }
     }
-    if (t + 1 < t1) {
-      if (NBUF == 1) {
-        __syncthreads();
-        fetch(t + 1);
-      }
-      put(t + 1, NBUF == 2 && !((t - t0) & 1) ? smem + buffer : smem);
+    if (NBUF == 1 && t + 1 < t1) {
+      __syncthreads();
+      fetch(t + 1, smem);
     }
   }
 
@@ -387,7 +378,7 @@ static int key_splits(const AttnArgs& a) {
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
   auto kern = a.row4 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, true> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, false>;
-  const size_t smem = buffers<T>(MAPS * DQ + DV) * (Stage<T, DQ, DV, MAPS>::TILES + KEYS * 4 + (size_t)a.window * 4);
+  const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nq * a.splits)), dim3(64 * WAVES), smem, st, a);
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
