@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       fetch_tile<T, DV>(to + MAPS * QT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
       int* codes = reinterpret_cast<int*>(to + TILES);
       fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
-      if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
+      if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst);
     };
     __syncthreads();                                             // the image before this one is done with the buffers
     if (tiles) fetch(0, smem);
@@ -122,13 +122,13 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       const unsigned ring_base = (unsigned)base % size;
       const char *Ks = at, *Vs = at + MAPS * QT;
       const int* kc = reinterpret_cast<const int*>(at + TILES);
-      const float* win = reinterpret_cast<const float*>(kc + KEYS);
+      const unsigned win = window_place(reinterpret_cast<const float*>(kc + KEYS), aoff);
       if (busy)
 #pragma unroll 1
       for (int sub = 0; sub < 2; ++sub) {
         if (sub * 32 >= valid) break;
         float bias[16];
-        window_bias<ROW4>(bias, win, kc + sub * 32, aoff, half);
+        window_bias<ROW4>(bias, win, kc + sub * 32, half);
         // one map: the accumulators start at -D, the product ends at dP - D
         f32x16 dp = splat16(MAPS == 1 ? -del[0] : 0.f), s[MAPS];
 #pragma unroll
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
           for (int g = 0; g < 4; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const unsigned at = ring_base + kc[sub * 32 + 8 * g + 4 * half + (ROW4 ? 0 : e)] + aoff;                  // < 2 size
+              const unsigned at = ring_base + (unsigned)kc[sub * 32 + 8 * g + 4 * half + (ROW4 ? 0 : e)] / 4 + aoff;    // < 2 size
               __hip_atomic_fetch_add(my_ring + min(at, at - size) + (ROW4 ? e : 0), (double)bias[4 * g + e], __ATOMIC_RELAXED,
                                      __HIP_MEMORY_SCOPE_WORKGROUP);
             }
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
       load4_to_lds(lane < valid ? from + ((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + lane : attn_fill + (which < MAPS ? 4 : 0), rows + which * KEYS);
     }
     fetch_window(rows + 2 * MAPS * KEYS + 4, line + code_first - code_last + a.line_off, code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1);
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = code_last - grid_code(a.q_start + i0 + min((int)threadIdx.x, valid - 1), a.gw);   // falls along the row
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (code_last - grid_code(a.q_start + i0 + min((int)threadIdx.x, valid - 1), a.gw));   // falls along the row
   };
   if (tiles) fetch(0, smem);
   for (int t = 0; t < tiles; ++t) {
@@ -285,14 +285,14 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     const char *Qs = at, *Gs = at + MAPS * QT;
     const int* qc = reinterpret_cast<const int*>(at + TILES);
     const float* rows = reinterpret_cast<const float*>(qc + KEYS);
-    const float* win = rows + 2 * MAPS * KEYS + 4;
+    const unsigned win = window_place(rows + 2 * MAPS * KEYS + 4, koff);
     const int valid = min(a.Lq - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
       if (sub * 32 >= valid) break;
       float bias[16];
-      window_bias<ROW4, -1>(bias, win, qc + sub * 32, koff, half);
+      window_bias<ROW4, -1>(bias, win, qc + sub * 32, half);
       f32x16 dp = zero16(), s[MAPS], mix;
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {

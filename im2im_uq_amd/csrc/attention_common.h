@@ -71,10 +71,13 @@ template <> struct Mma<bf16_t> {
     return __builtin_bit_cast(short8, r);
   }
   static __device__ __forceinline__ Frag pack_rest(const f32x16& s, Frag hi, int t) {   // what pack() rounded away
-    const bf16x8 h = as_bf16x8(hi);
+    const u32x4 h = __builtin_bit_cast(u32x4, hi);
     bf16x8 r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = (__bf16)(s[8 * t + e] - (float)h[e]);
+    for (int e = 0; e < 4; ++e) {
+      r[2 * e] = (__bf16)(s[8 * t + 2 * e] - __uint_as_float(h[e] << 16));
+      r[2 * e + 1] = (__bf16)(s[8 * t + 2 * e + 1] - __uint_as_float(h[e] & 0xffff0000u));
+    }
     return __builtin_bit_cast(short8, r);
   }
   static __device__ __forceinline__ float dot(Frag f, const float* x, float acc) {
@@ -149,11 +152,16 @@ template <typename T, int D> __device__ __forceinline__ void load_row_frags(type
 // behind the last, elements behind a row) or infinite comes from here.  A masked row may hold anything, infinities and NaN too: a zero
 // probability does not silence them in a product, a zero operand does.
 static __device__ const float attn_fill[8] = {0.f, 0.f, 0.f, 0.f, INFINITY, INFINITY, INFINITY, INFINITY};
-__device__ __forceinline__ void load16_to_lds(const void* from, void* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// Written as assembly: behind the builtin the compiler waits for every such load before the next transposed LDS read, which is the prefetch
+// lost (the instructions have no result in registers; lds_loads_done() is their wait).
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
 }
-__device__ __forceinline__ void load4_to_lds(const void* from, void* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+__device__ __forceinline__ void load16_to_lds(const void* from, const void* to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_address(to)), "v"(from) : "memory");
+}
+__device__ __forceinline__ void load4_to_lds(const void* from, const void* to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_address(to)), "v"(from) : "memory");
 }
 // every load of this wave into LDS is there; before the barrier behind which others read it
 __device__ __forceinline__ void lds_loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt 0
@@ -181,20 +189,22 @@ __device__ __forceinline__ void fetch_window(float* to, const float* line, int n
 template <typename T> __host__ __device__ constexpr int buffers(int elements) { return elements * (int)sizeof(T) <= 512 ? 2 : 1; }
 template <typename T> __host__ __device__ constexpr size_t tile_bytes(int elements) { return (size_t)KEYS * elements * sizeof(T); }
 
-// the bias of a lane's 16 scores: places codes[row] + off of the window.  ROW4: four rows' codes are consecutive (rising or falling), one place
-// serves them; behind the last valid row that may reach three places over the window's end, values that the callers mask.
-template <bool ROW4, int STEP = 1> __device__ __forceinline__ void window_bias(float* bias, const float* win, const int* codes, int off, int half) {
+// the bias of a lane's 16 scores: at bytes codes[row] from the lane's own place in the window.  ROW4: four rows' codes are consecutive (rising or
+// falling), one place serves them; behind the last valid row that may reach three places over the window's end, values that the callers mask.
+typedef const __attribute__((address_space(3))) float* lds_floats;
+__device__ __forceinline__ unsigned window_place(const float* win, int off) {
+  unsigned p = lds_address(win) + 4 * off;
+  asm("" : "+v"(p));                                             // one register, not the window's place added again to each read
+  return p;
+}
+template <bool ROW4, int STEP = 1> __device__ __forceinline__ void window_bias(float* bias, unsigned place, const int* codes, int half) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if constexpr (ROW4) {
-      const float* w = win + codes[8 * g + 4 * half] + off;
+  for (int g = 0; g < 4; ++g)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bias[4 * g + e] = w[STEP * e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bias[4 * g + e] = win[codes[8 * g + 4 * half + e] + off];
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (ROW4) bias[4 * g + e] = ((lds_floats)(uintptr_t)(place + codes[8 * g + 4 * half]))[STEP * e];
+      else bias[4 * g + e] = *(lds_floats)(uintptr_t)(place + codes[8 * g + 4 * half + e]);
     }
-  }
 }
 
 // four consecutive elements (16 bytes of fp32, 8 bytes of bf16)

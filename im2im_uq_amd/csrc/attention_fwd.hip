@@ -96,7 +96,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
     fetch_tile<T, DV>(to + MAPS * KT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
     int* codes = reinterpret_cast<int*>(to + TILES);
     fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst;
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst);
   };
   if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; ++t) {
@@ -106,14 +106,14 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
     if (NBUF == 2 && t + 1 < t1) fetch(t + 1, (t - t0) & 1 ? smem : smem + buffer);
     const char *Ks = at, *Vs = at + MAPS * KT;
     const int* kc = reinterpret_cast<const int*>(at + TILES);
-    const float* win = reinterpret_cast<const float*>(kc + KEYS);
+    const unsigned win = window_place(reinterpret_cast<const float*>(kc + KEYS), aoff);
     const int valid = min(len - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
     for (int sub = 0; sub < 2; ++sub) {
       if (sub * 32 >= valid) break;
       float bias[16];
-      window_bias<ROW4>(bias, win, kc + sub * 32, aoff, half);
+      window_bias<ROW4>(bias, win, kc + sub * 32, half);
       f32x16 s[MAPS];
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
