@@ -224,7 +224,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 // ---------------------------------------------------------------------------------------------- keys' and values' gradients
 // One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.
 template <typename T, int DQ, int DV, int MAPS, bool ROW4>
-__global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS == 1 ? 3 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
   constexpr int NBUF = buffers<T>(MAPS * DQ + DV);
