@@ -87,7 +87,7 @@ def _rows16(t):
         if t.is_contiguous():                                # heads are multiples of 16 bytes long
             return t
         e, strides = t.element_size(), t.stride()
-        if strides[-1] == 1 and all(s * e % 16 == 0 for s in strides[:-1]):
+        if strides[-1] == 1 and all(s * e % 16 == 0 for s in strides[:-1]) and strides[1] * e < 1 << 25:
             return t
     return _dense16(t)
 

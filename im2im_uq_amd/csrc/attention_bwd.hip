@@ -60,6 +60,11 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   if (BIAS)
     for (int w = threadIdx.x; w < 2 * WAVES * (int)copy; w += 64 * WAVES) ring[w] = 0.0;
 
+  TileFetch<T, DQ> kt;
+  TileFetch<T, DV> vt;
+  kt.prepare(a.ks[1]);
+  vt.prepare(a.vs[1]);
+  const bool full = a.d == DQ && a.dv == DV;
   const int b0 = group * a.group_images, b1 = min(b0 + a.group_images, a.B);
   for (int b = b0; b < b1; ++b) {
     const int64_t bh = (int64_t)b * a.H + h;
@@ -94,14 +99,24 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
     int done = line_begin;                                       // line places that are written
 
-    auto fetch = [&](int t, char* to) {
-      const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
+    Raster keys(0, a.gw);
+    auto fetch = [&](int t, char* to) {                          // tiles in their order
+      const int j0 = t * KEYS, valid = min(len - j0, KEYS);
+      const T *k = kp + (int64_t)j0 * a.ks[1], *v = vp + (int64_t)j0 * a.vs[1];
+      if (full && valid == KEYS) {
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * QT, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
-      fetch_tile<T, DV>(to + MAPS * QT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+        for (int m = 0; m < MAPS; ++m) kt.whole(to + m * QT, k + m * a.ks[2]);
+        vt.whole(to + MAPS * QT, v);
+      } else {
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m) kt.part(to + m * QT, k + m * a.ks[2], a.ks[1], valid, a.d);
+        vt.part(to + MAPS * QT, v, a.vs[1], valid, a.dv);
+      }
+      const int code = keys.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
+      keys.next();
       int* codes = reinterpret_cast<int*>(to + TILES);
-      fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
-      if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst);
+      fetch_window(reinterpret_cast<float*>(codes + KEYS), line + first - code_last + a.line_off, last - first + qspan + 1);
+      if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (min(code, last) - first);
     };
     __syncthreads();                                             // the image before this one is done with the buffers
     if (tiles) fetch(0, smem);
@@ -261,11 +276,25 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
   const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(MAPS * h) * a.qs[2];
   const T* gp = static_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * a.dv;
   const int tiles = k0 < len ? (a.Lq + KEYS - 1) / KEYS : 0;
-  auto fetch = [&](int t, char* to) {
-    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS), code_last = grid_code(a.q_start + i0 + valid - 1, a.gw);
+  const int64_t gstride = (int64_t)a.H * a.dv;
+  TileFetch<T, DQ> qt;
+  TileFetch<T, DV> gt;
+  qt.prepare(a.qs[1]);
+  gt.prepare(gstride);
+  const bool full = a.d == DQ && a.dv == DV;
+  Raster queries(a.q_start, a.gw);
+  auto fetch = [&](int t, char* to) {                             // tiles in their order
+    const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS);
+    const T *q = qp + (int64_t)i0 * a.qs[1], *g = gp + (int64_t)i0 * gstride;
+    if (full && valid == KEYS) {
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * QT, qp + (int64_t)i0 * a.qs[1] + m * a.qs[2], a.qs[1], valid, a.d);
-    fetch_tile<T, DV>(to + MAPS * QT, gp + (int64_t)i0 * a.H * a.dv, (int64_t)a.H * a.dv, valid, a.dv);
+      for (int m = 0; m < MAPS; ++m) qt.whole(to + m * QT, q + m * a.qs[2]);
+      gt.whole(to + MAPS * QT, g);
+    } else {
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) qt.part(to + m * QT, q + m * a.qs[2], a.qs[1], valid, a.d);
+      gt.part(to + MAPS * QT, g, gstride, valid, a.dv);
+    }
     int* codes = reinterpret_cast<int*>(to + TILES);
     float* rows = reinterpret_cast<float*>(codes + KEYS);
     const int which = wave_index();                              // a wave fetches log-sums (infinite behind the last query: P = 0) or D of a map
@@ -273,8 +302,10 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
       const float* from = which < MAPS ? a.lse : a.delta;
       load4_to_lds(lane < valid ? from + ((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + lane : attn_fill + (which < MAPS ? 4 : 0), rows + which * KEYS);
     }
-    fetch_window(rows + 2 * MAPS * KEYS + 4, line + code_first - code_last + a.line_off, code_last - grid_code(a.q_start + i0, a.gw) + kspan + 1);
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (code_last - grid_code(a.q_start + i0 + min((int)threadIdx.x, valid - 1), a.gw));   // falls along the row
+    const int code = queries.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
+    queries.next();
+    fetch_window(rows + 2 * MAPS * KEYS + 4, line + code_first - last + a.line_off, last - first + kspan + 1);
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (last - min(code, last));   // falls along the row
   };
   if (tiles) fetch(0, smem);
   for (int t = 0; t < tiles; ++t) {

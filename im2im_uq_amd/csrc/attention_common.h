@@ -167,17 +167,57 @@ __device__ __forceinline__ void load4_to_lds(const void* from, const void* to) {
 __device__ __forceinline__ void lds_loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt 0
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// KEYS rows of a tile, by the whole workgroup
-template <typename T, int D> __device__ __forceinline__ void fetch_tile(char* to, const T* src, int64_t stride, int valid, int d) {
-  constexpr int BYTES = D * (int)sizeof(T), PR = BYTES / 16, V = 16 / (int)sizeof(T);
-  const int lane = threadIdx.x & 63, wave = wave_index();
-#pragma unroll
-  for (int n = 0; n < KEYS * PR / (64 * WAVES); ++n) {
-    const int i = (n * WAVES + wave) * 64 + lane, r = i / PR;
-    const int c = ((place<BYTES>(r & 15, i % PR) - (r & 15) * BYTES) >> 4) * V;              // the piece that lies here
-    load16_to_lds(r < valid && c < d ? static_cast<const void*>(src + r * stride + c) : attn_fill, to + (n * WAVES + wave) * 1024);
-  }
+__device__ __forceinline__ void load16_to_lds(const void* base, unsigned offset, const void* to) {       // uniform base, bytes of the lane from there
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(lds_address(to)), "s"(base), "v"(offset) : "memory");
 }
+
+// KEYS rows of a tile, by the whole workgroup.  A lane's places are the same for every tile: their offsets are kept (64 rows of a tensor are
+// within 2 GiB, attn_check).  Tiles with rows or elements to be zeroed choose an address for each piece.
+template <typename T, int D> struct TileFetch {
+  static constexpr int BYTES = D * (int)sizeof(T), PR = BYTES / 16, V = 16 / (int)sizeof(T), N = KEYS * PR / (64 * WAVES);
+  unsigned offset[N];
+  __device__ __forceinline__ static int piece_row(int n) { return ((n * WAVES + wave_index()) * 64 + ((int)threadIdx.x & 63)) / PR; }
+  __device__ __forceinline__ static int piece_column(int n) {                                  // the piece that lies there
+    const int r = piece_row(n) & 15;
+    return ((place<BYTES>(r, (threadIdx.x & 63) % PR) - r * BYTES) >> 4) * V;
+  }
+  __device__ __forceinline__ void prepare(int64_t stride) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) offset[n] = (unsigned)(piece_row(n) * stride + piece_column(n)) * (unsigned)sizeof(T);
+  }
+  __device__ __forceinline__ void whole(char* to, const T* src) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) load16_to_lds(src, offset[n], to + (n * WAVES + wave_index()) * 1024);
+  }
+  __device__ __forceinline__ static void part(char* to, const T* src, int64_t stride, int valid, int d) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = piece_row(n), c = piece_column(n);
+      load16_to_lds(r < valid && c < d ? static_cast<const void*>(src + r * stride + c) : attn_fill, to + (n * WAVES + wave_index()) * 1024);
+    }
+  }
+};
+
+// the code of the token at lane l of a tile of 64, tile after tile without a division
+struct Raster {
+  int row, col, step_row, step_col, gw;
+  __device__ __forceinline__ Raster(int first, int gw_) : gw(gw_) {
+    const int t = first + (threadIdx.x & 63);
+    row = t / gw;
+    col = t % gw;
+    step_row = KEYS / gw;
+    step_col = KEYS % gw;
+  }
+  __device__ __forceinline__ int code() const { return row * (2 * gw - 1) + col; }
+  __device__ __forceinline__ void next() {
+    row += step_row;
+    col += step_col;
+    if (col >= gw) {
+      col -= gw;
+      ++row;
+    }
+  }
+};
 
 // `n` floats of the line, in whole runs of 64 (the window's size in LDS is a multiple of that)
 __device__ __forceinline__ void fetch_window(float* to, const float* line, int n) {

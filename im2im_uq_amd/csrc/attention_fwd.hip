@@ -89,14 +89,29 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
   const float* line = a.line + (int64_t)h * a.line_len;
 
-  auto fetch = [&](int t, char* to) {
-    const int j0 = t * KEYS, valid = min(len - j0, KEYS), kfirst = grid_code(j0, a.gw);
+  TileFetch<T, DQ> kt;
+  TileFetch<T, DV> vt;
+  kt.prepare(a.ks[1]);
+  vt.prepare(a.vs[1]);
+  const bool full = a.d == DQ && a.dv == DV;
+  Raster keys(t0 * KEYS, a.gw);
+  auto fetch = [&](int t, char* to) {                             // tiles in their order
+    const int j0 = t * KEYS, valid = min(len - j0, KEYS);
+    const T *k = kp + (int64_t)j0 * a.ks[1], *v = vp + (int64_t)j0 * a.vs[1];
+    if (full && valid == KEYS) {
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) fetch_tile<T, DQ>(to + m * KT, kp + (int64_t)j0 * a.ks[1] + m * a.ks[2], a.ks[1], valid, a.d);
-    fetch_tile<T, DV>(to + MAPS * KT, vp + (int64_t)j0 * a.vs[1], a.vs[1], valid, a.dv);
+      for (int m = 0; m < MAPS; ++m) kt.whole(to + m * KT, k + m * a.ks[2]);
+      vt.whole(to + MAPS * KT, v);
+    } else {
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) kt.part(to + m * KT, k + m * a.ks[2], a.ks[1], valid, a.d);
+      vt.part(to + MAPS * KT, v, a.vs[1], valid, a.dv);
+    }
+    const int code = keys.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
+    keys.next();
     int* codes = reinterpret_cast<int*>(to + TILES);
-    fetch_window(reinterpret_cast<float*>(codes + KEYS), line + kfirst - code_last + a.line_off, grid_code(j0 + valid - 1, a.gw) - kfirst + qspan + 1);
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (grid_code(j0 + min((int)threadIdx.x, valid - 1), a.gw) - kfirst);
+    fetch_window(reinterpret_cast<float*>(codes + KEYS), line + first - code_last + a.line_off, last - first + qspan + 1);
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (min(code, last) - first);
   };
   if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; ++t) {
@@ -348,6 +363,7 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   const int64_t* st[3] = {p->q_stride, p->k_stride, p->v_stride};
   for (int t = 0; t < 3; ++t) {
     IM2IM_REQUIRE((reinterpret_cast<uintptr_t>(ptr[t]) & 15) == 0);
+    IM2IM_REQUIRE(st[t][1] * e * KEYS < (1ll << 31));
     for (int x = 0; x < 3; ++x) IM2IM_REQUIRE(st[t][x] >= 0 && (st[t][x] * e) % 16 == 0);
   }
   a->q = p->q; a->k = p->k; a->v = p->v;
