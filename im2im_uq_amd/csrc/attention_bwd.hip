@@ -22,6 +22,31 @@ template <bool ROW4> __device__ __forceinline__ double take_place(double* ring, 
   return s;
 }
 
+// ... and into the workgroup's line (places in front of it belong to queries that are not there)
+__device__ __forceinline__ void put_place(float* line, int at, double s, bool first) {
+  if (at >= 0) line[at] = first ? (float)s : line[at] + (float)s;
+}
+
+// a neighbour's value, zero over the ends of 16 lanes
+__device__ __forceinline__ float from_lane_before(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x111, 0xf, 0xf, true));                 // row_shr:1
+}
+template <int N> __device__ __forceinline__ float from_lane_behind(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x100 + N, 0xf, 0xf, true));             // row_shl:N
+}
+
+// accumulators of two waves that share their columns: the second puts its own into LDS, the first adds them
+template <int N> __device__ __forceinline__ void join_halves(f32x16* acc, float* box, int kw, bool put) {
+  if (put != (kw == 1)) return;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (put) box[(n * 16 + r) * 64] = acc[n][r];
+      else acc[n][r] += box[(n * 16 + r) * 64];
+    }
+}
+
 // -------------------------------------------------------------------------------------- queries' gradients, bias and lam
 // One workgroup: 128 queries of one head, of `group_images` images in turn, against their keys in tiles of 64.
 // Bias gradient: a pair's place in the line is code(j) - code(i) + off.  Within one instruction 32 lanes have 32 different queries and the
@@ -29,11 +54,11 @@ template <bool ROW4> __device__ __forceinline__ double take_place(double* ring, 
 // of copies and its additions are in program order: no order is left open.  A copy is a ring over the line's index: the places
 // that the following tiles cannot reach any more are summed over the copies and written, each once.  The copies are 64-bit:
 // ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 3xx us at 78 images of 20 x 20, 8 x 64.
-template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4>
+template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const size_t buffer = TILES + KEYS * 4 + (size_t)a.window * 4;       // tiles, codes, window
@@ -42,19 +67,22 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, gh_ = lin / a.nq, h = gh_ % a.H, group = gh_ / a.H;
   const int slot = group * a.nq + qt;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
-  const int i0 = qt * ROWS, i_last = min(i0 + ROWS, a.Lq) - 1;
+  const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
+  const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31), ic = min(i, i_last);
   const bool mine = i < a.Lq, busy = i0 + wave * 32 < a.Lq;
-  const int code_last = grid_code(a.q_start + i_last, a.gw);
-  const int aoff = code_last - grid_code(a.q_start + ic, a.gw);
+  const int code_last = grid_code(a.q_start + i0 + QR - 1, a.gw);      // of 32 columns for each wave, on behind the last query
+  const int aoff = code_last - grid_code(a.q_start + i, a.gw);
   const int qspan = code_last - grid_code(a.q_start + i0, a.gw);
   const float scale2 = a.scale * LOG2E, lam = MAPS == 2 ? a.lam[h] : 0.f;
   const float* line = a.line + (int64_t)h * a.line_len;
   const unsigned size = a.ring, copy = size + 4;
-  double* my_ring = ring + (wave * 2 + half) * copy;
+  double* my_ring = ring + (wave_index() * 2 + half) * copy;
   float* line_out = BIAS ? a.line_part + ((int64_t)slot * a.H + h) * a.line_len : nullptr;
-  const int line_begin = a.line_off - code_last, line_end = grid_code(a.Lk - 1, a.gw) - code_last + a.line_off + qspan + 1;
+  const int line_shift = a.line_off - code_last, places = grid_code(a.Lk - 1, a.gw) + qspan + 1;
+  // the last lane of a run: of queries side by side within 16 lanes
+  const bool run_end = (lane & 15) == 15 || (a.q_start + i + 1) % a.gw == 0;
+  const bool run_tail = run_end || (lane & 15) >= 13 || (a.q_start + i + 2) % a.gw == 0 || (a.q_start + i + 3) % a.gw == 0;
   float dlam = 0.f;
 
   if (BIAS)
@@ -89,7 +117,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       }
       d += __shfl_xor(d, 32);
       del[m] = m == 0 ? d : -lam * d;
-      if (mine && half == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
+      if (mine && half == 0 && kw == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
 #pragma unroll
       for (int n = 0; n < DQ / 32; ++n) acc[m][n] = zero16();
     }
@@ -97,7 +125,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
     const int tiles = (len + KEYS - 1) / KEYS;
     const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)(MAPS * h) * a.ks[2];
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
-    int done = line_begin;                                       // line places that are written
+    int done = 0;                                                // places (line places from line_shift on) that are written
 
     Raster keys(0, a.gw);
     auto fetch = [&](int t, char* to) {                          // tiles in their order
@@ -115,20 +143,20 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       const int code = keys.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
       keys.next();
       int* codes = reinterpret_cast<int*>(to + TILES);
-      fetch_window(reinterpret_cast<float*>(codes + KEYS), line + first - code_last + a.line_off, last - first + qspan + 1);
+      fetch_window(reinterpret_cast<float*>(codes + KEYS), line, a.line_len, first - code_last + a.line_off, last - first + qspan + 1);
       if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (min(code, last) - first);
     };
     __syncthreads();                                             // the image before this one is done with the buffers
     if (tiles) fetch(0, smem);
     for (int t = 0; t < tiles; ++t) {
-      const int base = grid_code(t * KEYS, a.gw) - code_last + a.line_off, valid = min(len - t * KEYS, KEYS);
+      const int base = grid_code(t * KEYS, a.gw), valid = min(len - t * KEYS, KEYS);
       char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
       lds_loads_done();
       __syncthreads();
       if (BIAS && done < base) {                                 // a place's thread is the same for every image
         for (int w = done + ((int)threadIdx.x - done & 255); w < base; w += 64 * WAVES) {
           const double s = take_place<ROW4>(ring, (unsigned)w % size, size);
-          line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
+          put_place(line_out, w + line_shift, s, b == b0);
         }
         done = base;
         if (!a.ring_wide) __syncthreads();                       // else the places that this tile adds to are others
@@ -140,7 +168,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       const unsigned win = window_place(reinterpret_cast<const float*>(kc + KEYS), aoff);
       if (busy)
 #pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
+      for (int sub = kw; sub < 2; sub += KS) {
         if (sub * 32 >= valid) break;
         float bias[16];
         window_bias<ROW4>(bias, win, kc + sub * 32, half);
@@ -181,13 +209,27 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
         }
         if (BIAS) {
 #pragma unroll
-          for (int g = 0; g < 4; ++g)
+          for (int g = 0; g < 4; ++g) {
+            const int* code = kc + sub * 32 + 8 * g + 4 * half;
+            if constexpr (ROW4) {
+              // Four keys side by side: the pairs (i, j + e) and (i + 1, j + e + 1) share a place, so they are summed from lane to lane first, and
+              // four additions to LDS become one and, at the end of a run, where the sums that have no next lane lie, another.
+              const float d0 = bias[4 * g], d1 = bias[4 * g + 1] + from_lane_before(run_end ? 0.f : d0);
+              const float d2 = bias[4 * g + 2] + from_lane_before(run_end ? 0.f : d1);
+              const float d3 = bias[4 * g + 3] + from_lane_before(run_end ? 0.f : d2);
+              const float tail = (run_end ? d0 : 0.f) + from_lane_behind<1>(run_end ? d1 : 0.f) + from_lane_behind<2>(run_end ? d2 : 0.f);
+              const unsigned at = ring_base + (unsigned)code[0] / 4 + aoff;                                        // < 2 size
+              double* to = my_ring + min(at, at - size);
+              __hip_atomic_fetch_add(to + 3, (double)d3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              if (run_tail) __hip_atomic_fetch_add(to, (double)tail, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const unsigned at = ring_base + (unsigned)kc[sub * 32 + 8 * g + 4 * half + (ROW4 ? 0 : e)] / 4 + aoff;    // < 2 size
-              __hip_atomic_fetch_add(my_ring + min(at, at - size) + (ROW4 ? e : 0), (double)bias[4 * g + e], __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+              for (int e = 0; e < 4; ++e) {
+                const unsigned at = ring_base + (unsigned)code[e] / 4 + aoff;
+                __hip_atomic_fetch_add(my_ring + min(at, at - size), (double)bias[4 * g + e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+              }
             }
+          }
         }
 #pragma unroll
         for (int ks = 0; ks < 32 / M::KC; ++ks)
@@ -206,12 +248,21 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 
     if (BIAS) {
       __syncthreads();
-      for (int w = done + ((int)threadIdx.x - done & 255); w < line_end; w += 64 * WAVES) {
+      for (int w = done + ((int)threadIdx.x - done & 255); w < places; w += 64 * WAVES) {
         const double s = w - done < a.ring ? take_place<ROW4>(ring, (unsigned)w % size, size) : 0.0;
-        line_out[w] = b == b0 ? (float)s : line_out[w] + (float)s;
+        put_place(line_out, w + line_shift, s, b == b0);
       }
     }
-    if (mine) {
+    if (KS == 2) {
+      float* box = reinterpret_cast<float*>(smem) + wave * (MAPS * DQ / 2 * 64) + lane;
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) join_halves<DQ / 32>(acc[m], box + m * (DQ / 2 * 64), kw, true);
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) join_halves<DQ / 32>(acc[m], box + m * (DQ / 2 * 64), kw, false);
+    }
+    if (mine && kw == 0) {
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
         T* dst = static_cast<T*>(a.dq) + b * a.dqs[0] + (int64_t)i * a.dqs[1] + (int64_t)(MAPS * h + m) * a.dqs[2];
@@ -230,7 +281,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 #pragma unroll
     for (int s = 32; s >= 1; s >>= 1) dlam += __shfl_xor(dlam, s);
     __syncthreads();
-    if (lane == 0) red[wave] = dlam;
+    if (lane == 0) red[wave_index()] = dlam;
     __syncthreads();
     if (threadIdx.x == 0) a.dlam_part[(int64_t)slot * a.H + h] = -(red[0] + red[1] + red[2] + red[3]);
   }
@@ -238,11 +289,11 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 
 // ---------------------------------------------------------------------------------------------- keys' and values' gradients
 // One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.
-template <typename T, int DQ, int DV, int MAPS, bool ROW4>
+template <typename T, int DQ, int DV, int MAPS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS == 1 ? 3 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // tiles, codes, [2][MAPS][KEYS] log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
@@ -251,9 +302,9 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
     *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
-  const int k0 = kt * ROWS, k_last = min(k0 + ROWS, a.Lk) - 1;
+  const int k0 = kt * QR, k_last = min(k0 + QR, a.Lk) - 1;
   const int j = k0 + wave * 32 + (lane & 31), jc = min(j, k_last);
   const bool mine = j < len, busy = k0 + wave * 32 < len;
   const int code_first = grid_code(k0, a.gw), koff = grid_code(jc, a.gw) - code_first, kspan = grid_code(k_last, a.gw) - code_first;
@@ -304,7 +355,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
     }
     const int code = queries.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
     queries.next();
-    fetch_window(rows + 2 * MAPS * KEYS + 4, line + code_first - last + a.line_off, last - first + kspan + 1);
+    fetch_window(rows + 2 * MAPS * KEYS + 4, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
     if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (last - min(code, last));   // falls along the row
   };
   if (tiles) fetch(0, smem);
@@ -320,7 +371,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
     const int valid = min(a.Lq - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = kw; sub < 2; sub += KS) {
       if (sub * 32 >= valid) break;
       float bias[16];
       window_bias<ROW4, -1>(bias, win, qc + sub * 32, half);
@@ -367,6 +418,18 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : sizeof(T) == 2 && MAPS 
       fetch(t + 1, smem);
     }
   }
+  if (KS == 2) {
+    float* box = reinterpret_cast<float*>(smem) + wave * ((MAPS * DQ + DV) / 2 * 64) + lane;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) join_halves<DQ / 32>(dk[m], box + m * (DQ / 2 * 64), kw, true);
+    join_halves<DV / 32>(dv, box + MAPS * (DQ / 2 * 64), kw, true);
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) join_halves<DQ / 32>(dk[m], box + m * (DQ / 2 * 64), kw, false);
+    join_halves<DV / 32>(dv, box + MAPS * (DQ / 2 * 64), kw, false);
+    if (kw == 1) return;
+  }
   if (j >= a.Lk) return;
   if (!mine) {                                                   // a key from lengths[b] on: zeros (its column has whatever its clamped place gave)
 #pragma unroll
@@ -405,7 +468,8 @@ __global__ __launch_bounds__(256) void attn_line_sum_kernel(const AttnArgs a, do
   double acc = 0.0;
   if (x < a.line_len)
     for (int qt = 0; qt < a.nq; ++qt) {
-      const int first = grid_code(a.q_start + qt * ROWS, a.gw), last = grid_code(a.q_start + min(qt * ROWS + ROWS, a.Lq) - 1, a.gw);
+      const int i0 = qt * (ROWS / a.ks_q);
+      const int first = grid_code(a.q_start + i0, a.gw), last = grid_code(a.q_start + min(i0 + ROWS / a.ks_q, a.Lq) - 1, a.gw);
       if (x < a.line_off - last || x > grid_code(a.Lk - 1, a.gw) - first + a.line_off) continue;
       for (int g = wave; g < a.groups; g += 4) acc += (double)a.line_part[((int64_t)(g * a.nq + qt) * a.H + h) * a.line_len + x];
     }
@@ -460,6 +524,12 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 // images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, in at most 256 MiB where one image a
 // workgroup would take more (several add to their line in memory, a read and a wait a tile)
 static void set_groups(AttnArgs* a) {
+  // half as many queries (keys) for each workgroup where there would be less than one workgroup a CU (fp32, 3 x 17x23 x 5 x 40: 66 -> 46 and
+  // 69 -> 44 us with 60 of them; with 320, 10 x 20x20 x 8 x 64 bf16, it costs: 39 -> 51 and 26 -> 27 us)
+  a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 256 ? 2 : 1;
+  a->ks_k = (int64_t)a->B * a->H * cdiv(a->Lk, ROWS) < 256 ? 2 : 1;
+  a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);
+  a->nk = (int)cdiv(a->Lk, ROWS / a->ks_k);
   const int64_t line = (int64_t)a->H * a->nq * a->line_len * 4;
   a->groups = (int)std::max<int64_t>(1, std::min<int64_t>(a->B, (256ll << 20) / line));
   a->group_images = (int)cdiv(a->B, a->groups);
@@ -478,8 +548,8 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   return l;
 }
 
-template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
-  auto kern = a.row4 ? attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, true> : attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, false>;
+template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
+  auto kern = a.ks_q == 2 ? attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, ROW4, 2> : attn_bwd_q_kernel<T, DQ, DV, MAPS, BIAS, ROW4, 1>;
   const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4) +
                       (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
@@ -487,13 +557,21 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS> static int launch_bwd
   return check_launch("attn_bwd_q_kernel");
 }
 
-template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, hipStream_t st) {
-  if (int rc = a.line_part ? launch_bwd_q<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false>(a, st)) return rc;
-  auto kern = a.row4 && a.q_start % 4 == 0 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, true> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, false>;
-  const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
+template <typename T, int DQ, int DV, int MAPS, bool ROW4> static int launch_bwd_kv(const AttnArgs& a, hipStream_t st) {
+  auto kern = a.ks_k == 2 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 2> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 1>;
+  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
+  if (a.ks_k == 2) smem = std::max<size_t>(smem, (size_t)(MAPS * DQ + DV) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_kv_kernel");
+}
+
+template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, hipStream_t st) {
+  int rc;
+  if (a.line_part) rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, true, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, true, false>(a, st);
+  else rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, false, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false, false>(a, st);
+  if (rc) return rc;
+  return a.row4q ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
 }
 
 template <typename T> static int dispatch_bwd(const AttnArgs& a, int maps, hipStream_t st) {

@@ -2,7 +2,7 @@
 //
 // Tokens are the pixels of a gh x gw grid in raster order.  With code(t) = (t / gw) * (2 gw - 1) + t % gw the learned bias of a
 // (query i, key j) pair is line[code(j) - code(i) + off], off = code(gh gw - 1): one vector per head, expanded from the bucket table
-// (im2im_relpos_line), so a pair's bias is one subtraction and one LDS read, and its gradient one LDS add.
+// (im2im_relpos_line; a single row counts as one of endless width: code(t) = t), so a pair's bias is one subtraction and one LDS read, and its gradient one LDS add.
 //
 // MFMA shape: v_mfma_f32_32x32x16_bf16 (fp32: four v_mfma_f32_32x32x2_f32 per 16-byte fragment).  In the 32 x 32 result lane l holds column
 // l % 32 and rows row(r) = 8 (r / 4) + 4 (l / 32) + r % 4, r = 0..15.  Scores are computed TRANSPOSED (keys as rows, queries as
@@ -24,8 +24,9 @@ struct AttnArgs {
   const int32_t* lengths;             // [B] or null
   const float* lam;                   // [H] (two maps)
   int B, Lq, Lk, H, d, dv, gw, line_len, line_off, q_start, nq, nk;
+  int ks_q, ks_k;                     // waves that share 32 queries (keys): 1 or 2
   int window;                         // floats of LDS for the window of `line` that a tile reaches
-  int row4;                           // any four tokens from a multiple of four on lie side by side in the grid
+  int row4, row4q;                    // four keys (and queries) from a multiple of four on lie side by side in the grid
   float scale;                        // of the scores
   // forward
   void* out;                          // [B][Lq][H][dv]
@@ -219,10 +220,11 @@ struct Raster {
   }
 };
 
-// `n` floats of the line, in whole runs of 64 (the window's size in LDS is a multiple of that)
-__device__ __forceinline__ void fetch_window(float* to, const float* line, int n) {
+// `n` floats of the line from place `first` on, in whole runs of 64 (the window's size in LDS is a multiple of that).  The places of queries behind the
+// last one may lie in front of the line: any value will do there.
+__device__ __forceinline__ void fetch_window(float* to, const float* line, int line_len, int first, int n) {
   const int lane = threadIdx.x & 63;
-  for (int w = wave_index() * 64; w < n; w += 64 * WAVES) load4_to_lds(line + min(w + lane, n - 1), to + w);
+  for (int w = wave_index() * 64; w < n; w += 64 * WAVES) load4_to_lds(line + max(0, min(first + w + lane, line_len - 1)), to + w);
 }
 
 // LDS buffers of tiles: two (the next tile's loads run behind this tile's work, one barrier a tile), one for the widest heads in 32 bits
@@ -261,13 +263,8 @@ __device__ __forceinline__ int xcd_band(int id, int total) {
   return x * each + (x < more ? x : more) + (id >> 3);
 }
 
-// window of `line` that n consecutive tokens x KEYS tokens can reach, in floats
-inline int code_span(int64_t n, int gh, int gw) {
-  if (gh == 1) return (int)n - 1;
-  int64_t rows = (n - 1 + gw - 1) / gw;
-  if (rows > gh - 1) rows = gh - 1;
-  return (int)(n - 1 + rows * (gw - 1));
-}
+// distance in the line that n consecutive tokens span at most (also on behind the grid's last row)
+inline int code_span(int64_t n, int gh, int gw) { return (int)(gh == 1 ? n - 1 : n - 1 + (n - 1 + gw - 1) / gw * (gw - 1)); }
 inline int window_floats(int gh, int gw) { return code_span(ROWS, gh, gw) + code_span(KEYS, gh, gw) + 1; }
 inline int round64(int n) { return (n + 63) / 64 * 64; }
 

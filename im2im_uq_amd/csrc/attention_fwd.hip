@@ -40,7 +40,8 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------- forward
-// One workgroup: 128 queries (a wave has 32 of them as its columns), keys in tiles of 64 through LDS, a wave takes 32 of them at a time.
+// One workgroup: 128 queries (a wave has 32 of them as its columns), keys in tiles of 64 through LDS, a wave takes 32 of them at a time.  KS = 2: 64
+// queries, two waves share 32 and take one half of each tile's keys (joined at the end): for calls that would leave CUs without work.
 // The running maximum follows the scores only where they pass it by more than 2^GROW: until then probabilities up to 2^GROW are as exact in
 // 32 bits and in bf16 as those up to 1, and the accumulators need no rescaling (a handful of times a row).
 // SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
@@ -48,19 +49,19 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // cancellation, would carry a rounding of P to bf16 (2^-9) in every D.
 constexpr float GROW = 8.f;
 
-template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4>
-__global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
+template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS>
+__global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
+  constexpr int QR = ROWS / KS, NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t KT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const size_t buffer = TILES + KEYS * 4 + (size_t)a.window * 4;           // tiles, codes, window
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.splits, item = lin / a.splits;
   const int qt = item % a.nq, bh = item / a.nq, h = bh % a.H, b = bh / a.H;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
-  const int i0 = qt * ROWS, i_last = min(i0 + ROWS, a.Lq) - 1;
+  const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
+  const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31);
   const bool mine = i < a.Lq, busy = i0 + wave * 32 < a.Lq;
   const int code_last = grid_code(a.q_start + i_last, a.gw);
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
     const int code = keys.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
     keys.next();
     int* codes = reinterpret_cast<int*>(to + TILES);
-    fetch_window(reinterpret_cast<float*>(codes + KEYS), line + first - code_last + a.line_off, last - first + qspan + 1);
+    fetch_window(reinterpret_cast<float*>(codes + KEYS), line, a.line_len, first - code_last + a.line_off, last - first + qspan + 1);
     if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (min(code, last) - first);
   };
   if (t0 < t1) fetch(t0, smem);
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
     const int valid = min(len - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
-    for (int sub = 0; sub < 2; ++sub) {
+    for (int sub = kw; sub < 2; sub += KS) {
       if (sub * 32 >= valid) break;
       float bias[16];
       window_bias<ROW4>(bias, win, kc + sub * 32, half);
@@ -193,6 +194,35 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 1024 ? 1 : 2) 
     }
   }
 
+  if (KS == 2) {                                                  // the two waves of 32 queries, through LDS
+    float* box = reinterpret_cast<float*>(smem) + wave * (MAPS * (NB * 16 + 2) * 64) + lane;
+    __syncthreads();
+    if (kw == 1) {
+#pragma unroll
+      for (int m = 0; m < MAPS; ++m) {
+        float* to = box + m * (NB * 16 + 2) * 64;
+        to[0] = mx[m];
+        to[64] = sum[m];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) to[(2 + n * 16 + r) * 64] = o[m][n][r];
+      }
+    }
+    __syncthreads();
+    if (kw == 1) return;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) {
+      const float* from = box + m * (NB * 16 + 2) * 64;
+      const float top = fmaxf(mx[m], from[0]), ref = top == -INFINITY ? 0.f : top, w0 = exp2_(mx[m] - ref), w1 = exp2_(from[0] - ref);
+      mx[m] = top;
+      sum[m] = sum[m] * w0 + from[64] * w1;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[m][n][r] = o[m][n][r] * w0 + from[(2 + n * 16 + r) * 64] * w1;
+    }
+  }
   if (!busy) return;
   const int64_t row = (int64_t)bh * a.Lq + i;
 #pragma unroll
@@ -369,17 +399,24 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   a->q = p->q; a->k = p->k; a->v = p->v;
   for (int x = 0; x < 3; ++x) { a->qs[x] = p->q_stride[x]; a->ks[x] = p->k_stride[x]; a->vs[x] = p->v_stride[x]; }
   a->line = p->line; a->lengths = p->lengths; a->lam = p->lam;
-  a->B = p->B; a->Lq = p->Lq; a->Lk = p->Lk; a->H = p->H; a->d = p->D; a->dv = p->D * p->maps; a->gw = p->gw;
+  a->B = p->B; a->Lq = p->Lq; a->Lk = p->Lk; a->H = p->H; a->d = p->D; a->dv = p->D * p->maps;
+  a->gw = p->gh == 1 ? 1 << 25 : p->gw;
   a->line_len = (2 * p->gh - 1) * (2 * p->gw - 1);
   a->line_off = (p->gh - 1) * (2 * p->gw - 1) + p->gw - 1;
   a->q_start = p->q_start;
   a->row4 = p->gh == 1 || p->gw % 4 == 0;
-  a->nq = (int)cdiv(p->Lq, ROWS);
+  a->row4q = a->row4 && p->q_start % 4 == 0;
   a->nk = (int)cdiv(p->Lk, ROWS);
   a->scale = p->scale;
   a->window = round64(window_floats(p->gh, p->gw) + 4);            // a run of four may reach three over the end
   IM2IM_REQUIRE((int64_t)p->B * p->H * p->Lq < (1ll << 31) && (int64_t)p->B * p->H * a->nk < (1ll << 31) / 64);
   return IM2IM_OK;
+}
+
+// Half as many queries for each workgroup where there would be fewer than two workgroups a CU (23 -> 21 us for 320 of them: 10 x 20x20 x 8 x 64)
+static void set_queries(AttnArgs* a) {
+  a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 512 ? 2 : 1;
+  a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);
 }
 
 // Parts of the keys: with fewer workgroups than two for each of the 256 CUs the rest of the chip takes key tiles (a single token against
@@ -392,9 +429,10 @@ static int key_splits(const AttnArgs& a) {
   return (int)cdiv(tiles, cdiv(tiles, n));
 }
 
-template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
-  auto kern = a.row4 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, true> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, false>;
-  const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4);
+template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
+  auto kern = a.ks_q == 2 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, ROW4, 2> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, ROW4, 1>;
+  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4);
+  if (a.ks_q == 2) smem = std::max<size_t>(smem, 2 * MAPS * (DV / 2 + 2) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nq * a.splits)), dim3(64 * WAVES), smem, st, a);
   if (int rc = check_launch("attn_fwd_kernel")) return rc;
@@ -405,6 +443,10 @@ template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd
     return check_launch("attn_combine_kernel");
   }
   return IM2IM_OK;
+}
+
+template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
+  return a.row4 ? launch_fwd<T, DQ, DV, MAPS, SAVE, true>(a, st) : launch_fwd<T, DQ, DV, MAPS, SAVE, false>(a, st);
 }
 
 template <typename T, bool SAVE> static int dispatch_fwd(const AttnArgs& a, int maps, hipStream_t st) {
@@ -440,6 +482,7 @@ extern "C" int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int
 extern "C" int64_t im2im_attention_fwd_workspace_bytes(const im2im_attention_desc* p) {
   AttnArgs a = {};
   if (attn_check(p, &a)) return -1;
+  set_queries(&a);
   const int n = key_splits(a);
   return n < 2 ? 0 : (int64_t)n * a.B * a.H * a.Lq * p->maps * (a.dv + 2) * 4;
 }
@@ -450,6 +493,7 @@ extern "C" int im2im_attention_fwd(const im2im_attention_desc* p, void* out, flo
   if (int rc = attn_check(p, &a)) return rc;
   IM2IM_REQUIRE(out && (lse != nullptr) == (map_out != nullptr));
   a.out = out; a.lse = lse; a.osave = map_out;
+  set_queries(&a);
   a.splits = key_splits(a);
   a.tiles_per_split = (int)cdiv(cdiv(a.Lk, KEYS), a.splits);
   if (a.splits > 1) {
