@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 
 from ... import _pkg  # noqa: F401
+from .attention import AttentionBottleneck
 from .unet_parts import DoubleConv, Down, OutConv, Up, _cdt
 
 
@@ -29,7 +30,8 @@ def unet_plan(n_channels_in, depth=4, base=64, bilinear=True):
 
 
 class UNet(nn.Module):
-    def __init__(self, n_channels_in, n_channels_out, bilinear=True, depth=4, base=64, norm="batch"):
+    def __init__(self, n_channels_in, n_channels_out, bilinear=True, depth=4, base=64, norm="batch", attention=None, attention_blocks=1):
+        """attention: None (the reference's network), "relative" or "differential": that many AttentionBottleneck blocks on the deepest feature map"""
         super(UNet, self).__init__()
         self.n_channels_in, self.n_channels_middle, self.n_channels_out = n_channels_in, 32, n_channels_out
         self.bilinear = bilinear
@@ -42,6 +44,8 @@ class UNet(nn.Module):
             else:
                 setattr(self, name, Up(cin, cout, bilinear, norm=norm))
         self.out = OutConv(base, self.n_channels_middle)
+        # last, so that the other parameters are registered (and initialised) as without it
+        self.attention = AttentionBottleneck(base * 2 ** depth // (2 if bilinear else 1), attention, attention_blocks) if attention is not None else None
 
     def forward(self, x):
         if not self.training and not torch.is_grad_enabled():
@@ -73,7 +77,10 @@ class UNet(nn.Module):
         for i in range(1, depth):
             feat, pooled = getattr(self, f"down{i}")(pooled, lazy=True, pool=True, pooled=True)
             skips.append(feat)
-        h = getattr(self, f"down{depth}")(pooled, lazy=True, pooled=True)
+        attention = getattr(self, "attention", None)
+        h = getattr(self, f"down{depth}")(pooled, lazy=attention is None, pooled=True)
+        if attention is not None:
+            h = attention(h)
         for k in range(1, depth + 1):                                  # up1(x5, x4) ... up4(., x1)  (:40-43)
             h = getattr(self, f"up{k}")(h, skips[depth - k], lazy=True, tail=tail if k == depth else None)
         return h

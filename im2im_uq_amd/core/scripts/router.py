@@ -88,7 +88,7 @@ def run_experiment(params, dataset=None):
     if dataset is None:
         dataset = build_dataset(params)
     if params["model"] == "UNet":
-        trunk = UNet(params["num_inputs"], 1)
+        trunk = UNet(params["num_inputs"], 1, attention=params.get("attention"), attention_blocks=params.get("attention_blocks", 1))
     else:
         raise NotImplementedError
     model = add_uncertainty(trunk, params)

@@ -1614,15 +1614,15 @@ class ConvTranspose2x2(torch.autograd.Function):
 
 
 class Conv1x1(torch.autograd.Function):
-    """OutConv (unet_parts.py:87-94): 1x1 conv with bias on the MFMA kernel (taps = 1); input may be lazy."""
+    """OutConv (unet_parts.py:87-94): 1x1 conv with bias (or None) on the MFMA kernel (taps = 1); input may be lazy."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, cdt):
         ss = lazy_ss(x)
         xin = nhwc(x.detach(), cdt)
         wf, wd = packed_pair(weight, cdt)                     # with the 3x3 weights' per-step batch (one launch for the model)
-        y = conv_fwd(xin, wf, bias.detach(), in_ss=ss)
-        ctx.has_ss = ss is not None
+        y = conv_fwd(xin, wf, None if bias is None else bias.detach(), in_ss=ss)
+        ctx.has_ss, ctx.has_bias = ss is not None, bias is not None
         ctx.link = getattr(x, LINK_ATTR, None)
         ctx.save_for_backward(xin, wd, ss if ss is not None else torch.empty(0))
         return nchw(y)
@@ -1641,7 +1641,7 @@ class Conv1x1(torch.autograd.Function):
             else:
                 dx = nchw(conv_fwd(dy, wd))
         dw = conv_wgrad(xin, dy, 1, x_ss=ss).view(dy.shape[3], xin.shape[3], 1, 1)
-        return dx, dw, colsum(dy), None
+        return dx, dw, colsum(dy) if ctx.has_bias else None, None
 
 
 _HEADS_CACHE = WeakTensorKeyDictionary()     # first head weight -> (key, packed weights, concatenated biases): inference only
