@@ -46,13 +46,16 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // 32 bits and in bf16 as those up to 1, and the accumulators need no rescaling (a handful of times a row).
 // SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
 // result exact to about 2^-18: the backward's row sums D = dO . O are taken from it, and the table's gradient, a 32-bit sum with much
-// cancellation, would carry a rounding of P to bf16 (2^-9) in every D.
+// cancellation, would carry a rounding of P to bf16 (2^-9) in every D.  Without it, of two maps the first takes hi + lo (lam is mostly below one): their
+// difference is smaller than either, and both maps' roundings left 1.5 times the error of a result rounded once (1.15 so; both as hi + lo: 254 us
+// for 168 at 16 x 40x40 x 4 x 64).
 constexpr float GROW = 8.f;
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
+  constexpr int HILO = sizeof(T) == 4 ? 0 : SAVE ? MAPS : MAPS - 1;        // the first so many maps' probabilities as hi + lo
   constexpr int QR = ROWS / KS, NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t KT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -175,7 +178,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
           pf[m] = M::pack(s[m], ks);
-          if (SAVE && sizeof(T) == 2) pr[m] = M::pack_rest(s[m], pf[m], ks);
+          if (m < HILO) pr[m] = M::pack_rest(s[m], pf[m], ks);
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
           for (int m = 0; m < MAPS; ++m) {
             o[m][n] = M::mma(vf, pf[m], o[m][n]);
-            if (SAVE && sizeof(T) == 2) o[m][n] = M::mma(vf, pr[m], o[m][n]);
+            if (m < HILO) o[m][n] = M::mma(vf, pr[m], o[m][n]);
           }
         }
       }
