@@ -92,6 +92,11 @@ def _rows16(t):
     return _dense16(t)
 
 
+def _like(t):
+    """a dense tensor of t's shape (empty_like keeps strides that say nothing, zeros among them, of sizes of one)"""
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -228,7 +233,7 @@ class _GridAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, lengths, saved = ctx.saved_tensors
-        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        dq, dk, dv = _like(q), _like(k), _like(v)
         dtable, dlam = _backward(ctx.plan, q, k, v, saved, None if lam is None else lam.contiguous(), lengths, dout, dq, dk, dv, ctx.needs_input_grad[3])
         return dq, dk, dv, dtable, dlam, None, None
 

@@ -538,19 +538,13 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 
 // -------------------------------------------------------------------------------------------------------------------- host
 
-// images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own, in at most 256 MiB where one image a
-// workgroup would take more (several add to their line in memory, a read and a wait a tile)
-static void set_groups(AttnArgs* a) {
+static void set_tiles(AttnArgs* a) {
   // half as many queries (keys) for each workgroup where there would be less than one workgroup a CU (fp32, 3 x 17x23 x 5 x 40: 66 -> 46 and
   // 69 -> 44 us with 60 of them; with 320, 10 x 20x20 x 8 x 64 bf16, it costs: 39 -> 51 and 26 -> 27 us)
   a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 256 ? 2 : 1;
   a->ks_k = (int64_t)a->B * a->H * cdiv(a->Lk, ROWS) < 256 ? 2 : 1;
   a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);
   a->nk = (int)cdiv(a->Lk, ROWS / a->ks_k);
-  const int64_t line = (int64_t)a->H * a->nq * a->line_len * 4;
-  a->groups = (int)std::max<int64_t>(1, std::min<int64_t>(a->B, (256ll << 20) / line));
-  a->group_images = (int)cdiv(a->B, a->groups);
-  a->groups = (int)cdiv(a->B, a->group_images);
 }
 
 struct BwdLayout { int64_t delta, part, line, dlam, bytes; };
@@ -563,6 +557,18 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   l.dlam = l.part + (table ? up((int64_t)a.groups * a.nq * a.H * a.line_len * 4) : 0);
   l.bytes = l.dlam + up((int64_t)a.groups * a.nq * a.H * 4);
   return l;
+}
+
+// Images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own.  One image where that takes at
+// most 256 MiB and the workspace holds it (several add to their line in memory, a read and a wait a tile).
+static BwdLayout set_groups(AttnArgs* a, int maps, bool table, int64_t ws_bytes) {
+  int64_t groups = a->B;
+  if (table) groups = std::max<int64_t>(1, std::min<int64_t>(groups, (256ll << 20) / ((int64_t)a->H * a->nq * a->line_len * 4)));
+  for (a->group_images = (int)cdiv(a->B, groups);; ++a->group_images) {
+    a->groups = (int)cdiv(a->B, a->group_images);
+    const BwdLayout l = bwd_layout(*a, maps, table);
+    if (l.bytes <= ws_bytes || a->groups == 1) return l;
+  }
 }
 
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
@@ -605,8 +611,8 @@ using namespace im2im;
 extern "C" int64_t im2im_attention_bwd_workspace_bytes(const im2im_attention_desc* p, int32_t want_table) {
   AttnArgs a = {};
   if (attn_check(p, &a)) return -1;
-  set_groups(&a);
-  return bwd_layout(a, p->maps, want_table != 0).bytes;
+  set_tiles(&a);
+  return set_groups(&a, p->maps, want_table != 0, INT64_MAX).bytes;
 }
 
 extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_attention_grads* g, void* ws, int64_t ws_bytes,
@@ -627,8 +633,9 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   const bool table = g->dtable != nullptr;
   IM2IM_REQUIRE(!table || (g->ny >= 1 && g->ny <= 64 && (g->ny == 1 || g->ny % 2 == 0) && g->nx >= 1 && g->nx <= 64 && (g->nx == 1 || g->nx % 2 == 0)));
   IM2IM_REQUIRE(!table || ((g->ny <= 2 || g->thr_y) && (g->nx <= 2 || g->thr_x)));
-  set_groups(&a);
-  const BwdLayout l = bwd_layout(a, p->maps, table);
+  IM2IM_REQUIRE((int64_t)a.H * a.dv * e * KEYS < (1ll << 31));
+  set_tiles(&a);
+  const BwdLayout l = set_groups(&a, p->maps, table, ws_bytes);
   IM2IM_REQUIRE(ws && ws_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
   char* w = static_cast<char*>(ws);
   a.dout = g->dout; a.lse = const_cast<float*>(g->lse); a.osave = const_cast<float*>(g->map_out); a.delta = reinterpret_cast<float*>(w + l.delta);

@@ -63,6 +63,64 @@ def test_forward_and_gradients(maps, grid, b, heads, d, buckets, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,d", [(1, 32), (1, 64), (1, 80), (1, 128), (2, 24), (2, 32), (2, 64)])
+@pytest.mark.parametrize("grid,b", [((5, 7), 64), ((4, 8), 64), ((12, 12), 33), ((9, 15), 33)])
+def test_many_images(grid, b, maps, d, dtype):
+    """enough work for a workgroup of 128 queries or keys each (small calls share 32 of them between two waves), widths that are and are not a
+    multiple of four"""
+    o = operands(maps, dtype, grid, b, 8, d, (8, 8), seed=b + d)
+    lengths = torch.full((b,), grid[0] * grid[1], dtype=torch.int32, device=DEV)
+    lengths[1::3] = grid[0] * grid[1] // 2 + 1
+    lengths[2] = 0
+    want = reference(o, grid, lengths=lengths)
+    check(train(o, grid, lengths=lengths), want)
+    check({"out": call(o, grid, lengths=lengths)}, want, ("out",))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,d", [(1, 128), (2, 64)])
+def test_widest_grid(maps, d, dtype):
+    """512 wide: the largest window and accumulators in LDS"""
+    grid = (2, 512)
+    o = operands(maps, dtype, grid, 1, 1, d, (2, 64), seed=31)
+    check(train(o, grid, max_distance=300), reference(o, grid, max_distance=300))
+
+
+@pytest.mark.parametrize("maps,d", [(1, 32), (2, 32)])
+@pytest.mark.parametrize("grid", [(8, 12), (7, 9), (1, 300)])
+def test_small_workspace(grid, maps, d, monkeypatch):
+    """a workspace for fewer lines than images: workgroups take several images in turn and add to their line"""
+    o = operands(maps, BF16, grid, 7, 2, d, (8, 8), seed=33)
+    want = reference(o, grid)
+    lengths = torch.tensor([0, 40, 63, 5, 1, 64, 33], dtype=torch.int32, device=DEV)
+    want_ragged = reference(o, grid, lengths=lengths)
+    full = train(o, grid)
+    real = attn_ops.lib.im2im_attention_bwd
+    for images in (2, 3, 7):
+        def smaller(p, g, ws, n, stream, images=images):
+            line = 2 * (2 * grid[0] - 1) * (2 * grid[1] - 1) * 4 * ((grid[0] * grid[1] + 63) // 64)
+            return real(p, g, ws, n - (7 - -(-7 // images)) * (line - 256), stream)
+        monkeypatch.setattr(attn_ops.lib, "im2im_attention_bwd", smaller)
+        check(train(o, grid), want)
+        check(train(o, grid, lengths=lengths), want_ragged)
+    monkeypatch.undo()
+    assert all(torch.equal(full[n], t) for n, t in train(o, grid).items())
+
+
+def test_far_apart_rows():
+    """offsets that pass 32 bits: tokens 16 MiB apart"""
+    grid, step = (1, 300), 1 << 23
+    o = operands(1, BF16, grid, 1, 1, 32, (1, 8), seed=35)
+    far = torch.empty(300 * step, dtype=BF16, device=DEV)
+    s = dict(o)
+    for n, at in (("q", 0), ("k", 64), ("v", 128)):
+        s[n] = far.as_strided((1, 300, 1, 32), (300 * step, step, 32, 1), at)
+        s[n].copy_(o[n])
+    got, want = train(s, grid), train(o, grid)
+    assert s["k"].data_ptr() == far.data_ptr() + 128 and all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("maps,d", [(1, 64), (1, 40), (2, 32), (2, 64)])
 @pytest.mark.parametrize("lengths", [[0, 1, 63], [64, 65, 128], [129, 130, 1000], [130, -5, 64]])
 def test_lengths(maps, d, dtype, lengths):
@@ -143,6 +201,9 @@ def test_strides_and_alignment(maps):
              dout=o["dout"].transpose(1, 2).contiguous().transpose(1, 2))
     got = train(s, grid)
     assert all(torch.equal(got[n], dense[n]) for n in dense)
+    one = {n: t[:1].as_strided(t[:1].shape, (0, *t.stride()[1:])) if n in ("q", "k", "v") else None if t is None else t[:1] if n == "dout" else t
+           for n, t in o.items()}                            # a batch of one whose stride says nothing
+    assert torch.equal(train(one, grid)["dq"], dense["dq"][:1])
     s = dict(o, k=o["k"][:1].expand(3, -1, -1, -1), v=o["v"][..., ::2].repeat_interleave(2, -1)[..., ::2].repeat_interleave(2, -1))
     check(train(s, grid), reference(s, grid))
 
