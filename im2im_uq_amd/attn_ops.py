@@ -379,20 +379,21 @@ def _rows_of(t, shape):
 
 
 def _seam_desc(s, x, f, gate, params):
-    rows = [(None, 0) if t is None else (t[0].data_ptr(), t[1]) for t in (x, f, gate)]
-    return NormGateDesc(*(r[0] for r in rows), *(_ptr(t) for t in params), s.rows, *(r[1] for r in rows), s.c, s.norm, _DT[x[0].dtype], s.eps)
+    """the description of a call, its operands (they have to outlive the launch)"""
+    scale, post_weight, post_bias, pre_weight, pre_bias = params = [None if t is None else _dense16(t) for t in params]
+    (x, xs), (f, fs), (gate, gs) = rows = [(None, 0) if t is None else _rows_of(t, s.shape) for t in (x, f, gate)]
+    return NormGateDesc(x.data_ptr(), _ptr(f), _ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), s.rows, xs, fs, gs,
+                        s.c, s.norm, _DT[x.dtype], s.eps), (rows, params)
 
 
 def _seam_forward(s, x, f, gate, params):
-    x, f, gate = (None if t is None else _rows_of(t, s.shape) for t in (x, f, gate))
-    params = [None if t is None else _dense16(t) for t in params]
-    dev, dt = x[0].device, x[0].dtype
+    dev, dt = x.device, x.dtype
+    desc, operands = _seam_desc(s, x, f, gate, params)
     y = torch.empty(s.shape, dtype=dt, device=dev) if f is not None else None
     h = torch.empty(s.shape, dtype=dt, device=dev) if params[3] is not None else None
     guard = _guard(dev)
     try:
-        check(lib.im2im_norm_gate_fwd(ctypes.byref(_seam_desc(s, x, f, gate, params)), _ptr(y), _ptr(h), torch._C._cuda_getCurrentRawStream(dev.index)),
-              "im2im_norm_gate_fwd")
+        check(lib.im2im_norm_gate_fwd(ctypes.byref(desc), _ptr(y), _ptr(h), torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_norm_gate_fwd")
     finally:
         if guard is not None:
             guard.__exit__(None, None, None)
@@ -413,29 +414,38 @@ class _NormGate(torch.autograd.Function):
     def backward(ctx, *grads):
         s = ctx.s
         x, f, gate, *params = ctx.saved_tensors
-        has_y, has_h = f is not None, params[3] is not None
-        dy, dh = grads if has_y and has_h else (grads[0], None) if has_y else (None, grads[0])
+        dy, dh = grads if len(grads) == 2 else (grads[0], None) if f is not None else (None, grads[0])
         if dy is None and dh is None:
             return (None,) * 9
-        dev, dt = x.device, x.dtype
+        dev, dt, c = x.device, x.dtype, s.c
         dy, dh = (None if t is None else (t if t.dtype == dt else t.to(dt)).contiguous() for t in (dy, dh))
-        need = ctx.needs_input_grad[1:]
-        rows = [torch.empty(s.shape, dtype=dt, device=dev) if t is not None and n else None for t, n in zip((x, f, gate), need)]
-        want = [t is not None and n for t, n in zip(params, need[3:])]
-        sums = [torch.empty(s.c, dtype=F32, device=dev) if w and (i < 3 or dh is not None) else None for i, w in enumerate(want)]
-        params = [None if t is None else _dense16(t) for t in params]
-        n = lib.im2im_norm_gate_bwd_workspace_bytes(s.rows, s.c)
+        _, need_x, need_f, need_gate, *need = ctx.needs_input_grad
+        dx = torch.empty(s.shape, dtype=dt, device=dev) if need_x else None
+        df = torch.empty(s.shape, dtype=dt, device=dev) if need_f and f is not None else None
+        dgate = torch.empty(s.shape, dtype=dt, device=dev) if need_gate and gate is not None else None
+        want = [n and t is not None for n, t in zip(need, params)]
+        wanted = sum(want)
+        if wanted and c % 4 == 0:                            # one buffer, each row at 16 bytes
+            spare = list(torch.empty((wanted, c), dtype=F32, device=dev).unbind())
+        else:
+            spare = [torch.empty(c, dtype=F32, device=dev) for _ in range(wanted)]
+        sums = [spare.pop() if w else None for w in want]
+        if dh is None:                                       # no gradient came through the second norm
+            for t in sums[3:]:
+                if t is not None:
+                    t.zero_()
+        out = sums if dh is not None else [*sums[:3], None, None]
+        n = lib.im2im_norm_gate_bwd_workspace_bytes(s.rows, c)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        desc = _seam_desc(s, *(None if t is None else _rows_of(t, s.shape) for t in (x, f, gate)), params)
+        desc, operands = _seam_desc(s, x, f, gate, params)
         guard = _guard(dev)
         try:
-            check(lib.im2im_norm_gate_bwd(ctypes.byref(desc), _ptr(dy), _ptr(dh), *map(_ptr, rows), *map(_ptr, sums), ws.data_ptr(), n,
+            check(lib.im2im_norm_gate_bwd(ctypes.byref(desc), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(df), _ptr(dgate), *map(_ptr, out), ws.data_ptr(), n,
                                           torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_norm_gate_bwd")
         finally:
             if guard is not None:
                 guard.__exit__(None, None, None)
-        sums = [torch.zeros(s.c, dtype=F32, device=dev) if w and t is None else t for w, t in zip(want, sums)]
-        return (None, *rows, *sums)
+        return (None, dx, df, dgate, *sums)
 
 
 def norm_gate_residual(x, f, gate=None, scale=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, norm="rms", eps=1e-6):
