@@ -112,7 +112,8 @@ def _guard(device):
 
 class _Plan:
     """what a call is, beside its tensors: settled once for each combination of sizes (plain numbers only)"""
-    __slots__ = ("heads", "d", "maps", "desc", "sizes", "table_shape", "thr", "out_shape", "save", "fwd_ws", "bwd_ws", "line_at", "lse_at", "map_at")
+    __slots__ = ("heads", "d", "maps", "batch", "grid", "desc", "desc_qkv", "grads", "grads_qkv", "table_shape", "thr", "out_shape", "save", "fwd_ws",
+                 "bwd_ws", "lse_at", "map_at")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -149,47 +150,68 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
         _fail(f"scale must be finite, got {scale}")
     if b * lq and lk == 0:
         _fail("k, v: no keys (lengths may be 0, the tensors not)")
-    p.desc = None
+    p.desc, p.batch, p.grid = None, b, (gh, gw)
     if b * lq == 0:
         return p
-    # the description with the pointers left open, and the sizes that follow from it
+    # the description of dense operands with the pointers left open, and the sizes that follow from it
     t = p.desc = AttentionDesc()
     t.B, t.Lq, t.Lk, t.H, t.D, t.maps, t.gh, t.gw, t.q_start, t.dtype, t.scale = b, lq, lk, heads, d, maps, gh, gw, q_start, _DT[dtype], scale
     t.q = t.k = t.v = t.line = t.lam = 16
+    c = heads * maps * d
+    t.q_stride[:], t.k_stride[:], t.v_stride[:] = (lq * c, c, d), (lk * c, c, d), (lk * c, c, d * maps)
     p.fwd_ws = lib.im2im_attention_fwd_workspace_bytes(ctypes.byref(t))
     p.bwd_ws = [lib.im2im_attention_bwd_workspace_bytes(ctypes.byref(t), w) for w in (0, 1)]
     if p.fwd_ws < 0 or min(p.bwd_ws) < 0:
         check(-1, "im2im_attention_fwd")
-    # one buffer for the bias of every displacement and what the backward needs; places in floats, at 16 bytes
-    up = lambda n: (n + 3) // 4 * 4  # noqa: E731
-    p.line_at = 0
+    g = p.grads = AttentionGrads()
+    g.dq_stride[:], g.dk_stride[:], g.dv_stride[:] = t.q_stride, t.k_stride, t.v_stride
+    g.ny, g.nx = table_shape[:2]
+    g.thr_y, g.thr_x = (ctypes.cast(x, ctypes.c_void_p) for x in p.thr)
+    # the same for q, k and v side by side in one tensor
+    p.desc_qkv, p.grads_qkv = AttentionDesc.from_buffer_copy(t), AttentionGrads.from_buffer_copy(g)
+    for x in (p.desc_qkv.q_stride, p.desc_qkv.k_stride, p.grads_qkv.dq_stride, p.grads_qkv.dk_stride):
+        x[:] = 3 * lk * c, 3 * c, d
+    for x in (p.desc_qkv.v_stride, p.grads_qkv.dv_stride):
+        x[:] = 3 * lk * c, 3 * c, d * maps
+    # one buffer for the bias of every displacement (its begin) and what the backward needs; places in bytes, at 16
+    up = lambda n: (4 * n + 15) // 16 * 16  # noqa: E731
     p.lse_at = up(heads * (2 * gh - 1) * (2 * gw - 1))
     p.map_at = p.lse_at + up(b * heads * maps * lq)
-    p.save = p.map_at + b * heads * lq * maps * d * maps
+    p.save = p.map_at + up(b * heads * lq * maps * d * maps)
     return p
 
 
-def _describe(plan, q, k, v, line, lengths, lam):
+def _describe(plan, q, k, v, lengths, lam):
     p = AttentionDesc.from_buffer_copy(plan.desc)
-    p.q, p.k, p.v, p.line = q.data_ptr(), k.data_ptr(), v.data_ptr(), line
-    p.lengths, p.lam = _ptr(lengths), _ptr(lam)
-    p.q_stride[:], p.k_stride[:], p.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    p.q, p.k, p.v, p.lengths, p.lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), _ptr(lam)
+    if not q.is_contiguous():
+        p.q_stride[:] = q.stride()[:3]
+    if not k.is_contiguous():
+        p.k_stride[:] = k.stride()[:3]
+    if not v.is_contiguous():
+        p.v_stride[:] = v.stride()[:3]
     return p
 
 
-def _forward(plan, q, k, v, table, lam, lengths, keep):
-    """(out, saved): the buffer of the plan's line, log-sums and map results"""
-    dev = q.device
-    out = torch.empty(plan.out_shape, dtype=q.dtype, device=dev)
-    saved = torch.empty(plan.save if keep else plan.lse_at, dtype=F32, device=dev)
+def _describe_qkv(plan, qkv, lam):
+    p = AttentionDesc.from_buffer_copy(plan.desc_qkv)
+    at, step = qkv.data_ptr(), plan.heads * plan.maps * plan.d * qkv.element_size()
+    p.q, p.k, p.v, p.lam = at, at + step, at + 2 * step, _ptr(lam)
+    return p
+
+
+def _forward(plan, p, dtype, dev, table, keep):
+    """(out, saved) for the description `p` (its line is filled in): `saved` holds the line, log-sums and map results"""
+    out = torch.empty(plan.out_shape, dtype=dtype, device=dev)
+    saved = torch.empty(plan.save if keep else plan.lse_at, dtype=torch.uint8, device=dev)
     ws = torch.empty(plan.fwd_ws, dtype=torch.uint8, device=dev) if plan.fwd_ws else None
+    p.line = line = saved.data_ptr()
     guard = _guard(dev)
     try:
         stream = torch._C._cuda_getCurrentRawStream(dev.index)
-        line, t, shape = saved.data_ptr(), plan.desc, plan.table_shape
-        check(lib.im2im_relpos_line(table.data_ptr(), shape[0], shape[1], t.H, plan.thr[0], plan.thr[1], t.gh, t.gw, line, stream), "im2im_relpos_line")
-        p = _describe(plan, q, k, v, line, lengths, lam)
-        check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), line + 4 * plan.lse_at if keep else None, line + 4 * plan.map_at if keep else None,
+        ny, nx, heads = plan.table_shape
+        check(lib.im2im_relpos_line(table.data_ptr(), ny, nx, heads, plan.thr[0], plan.thr[1], plan.grid[0], plan.grid[1], line, stream), "im2im_relpos_line")
+        check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), line + plan.lse_at if keep else None, line + plan.map_at if keep else None,
                                       _ptr(ws), plan.fwd_ws, stream), "im2im_attention_fwd")
     finally:
         if guard is not None:
@@ -197,21 +219,20 @@ def _forward(plan, q, k, v, table, lam, lengths, keep):
     return out, saved
 
 
-def _backward(plan, q, k, v, saved, lam, lengths, dout, dq, dk, dv, want_table):
-    """fills dq, dk, dv ([B, L, heads, D] views); returns (dtable | None, dlam | None)"""
-    dev = q.device
-    dout = _dense16(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-    dtable = torch.empty(plan.table_shape, dtype=F32, device=dev) if want_table else None
-    dlam = torch.empty(plan.heads, dtype=F32, device=dev) if plan.maps == 2 else None
+def _backward(plan, p, g, saved, dout, want_table):
+    """launches the backward of the description `p`; `g` has the pointers of dq, dk, dv.  Returns (dtable | None, dlam | None)"""
+    dev = saved.device
+    line = saved.data_ptr()
+    dtable = dlam = None
+    g.dout, g.lse, g.map_out = dout.data_ptr(), line + plan.lse_at, line + plan.map_at
+    if want_table:
+        dtable = torch.empty(plan.table_shape, dtype=F32, device=dev)
+        g.dtable = dtable.data_ptr()
+    if plan.maps == 2:
+        dlam = torch.empty(plan.heads, dtype=F32, device=dev)
+        g.dlam = dlam.data_ptr()
     n = plan.bwd_ws[want_table]
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    line = saved.data_ptr()
-    g = AttentionGrads(dout.data_ptr(), line + 4 * plan.lse_at, line + 4 * plan.map_at, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(dlam))
-    g.dq_stride[:], g.dk_stride[:], g.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
-    if want_table:
-        g.ny, g.nx = plan.table_shape[:2]
-        g.thr_y, g.thr_x = (ctypes.cast(t, ctypes.c_void_p) for t in plan.thr)
-    p = _describe(plan, q, k, v, line, lengths, lam)
     guard = _guard(dev)
     try:
         check(lib.im2im_attention_bwd(ctypes.byref(p), ctypes.byref(g), ws.data_ptr(), n, torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_attention_bwd")
@@ -224,7 +245,9 @@ def _backward(plan, q, k, v, saved, lam, lengths, dout, dq, dk, dv, want_table):
 class _GridAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, lengths, plan):
-        out, saved = _forward(plan, q, k, v, table.contiguous(), None if lam is None else lam.contiguous(), lengths, True)
+        lam = None if lam is None else lam.contiguous()
+        p = _describe(plan, q, k, v, lengths, lam)
+        out, saved = _forward(plan, p, q.dtype, q.device, table.contiguous(), True)
         ctx.plan = plan
         ctx.save_for_backward(q, k, v, lam, lengths, saved)
         return out
@@ -233,8 +256,14 @@ class _GridAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, lengths, saved = ctx.saved_tensors
+        plan = ctx.plan
         dq, dk, dv = _like(q), _like(k), _like(v)
-        dtable, dlam = _backward(ctx.plan, q, k, v, saved, None if lam is None else lam.contiguous(), lengths, dout, dq, dk, dv, ctx.needs_input_grad[3])
+        p = _describe(plan, q, k, v, lengths, lam)
+        p.line = saved.data_ptr()
+        g = AttentionGrads.from_buffer_copy(plan.grads)
+        g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        dout = _dense16(dout)
+        dtable, dlam = _backward(plan, p, g, saved, dout, ctx.needs_input_grad[3])
         return dq, dk, dv, dtable, dlam, None, None
 
 
@@ -243,8 +272,9 @@ class _GridSelfAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, table, lam, plan):
-        qkv = _rows16(qkv)
-        out, saved = _forward(plan, *_split_qkv(qkv, plan), table.contiguous(), None if lam is None else lam.contiguous(), None, True)
+        qkv = _dense16(qkv)
+        lam = None if lam is None else lam.contiguous()
+        out, saved = _forward(plan, _describe_qkv(plan, qkv, lam), qkv.dtype, qkv.device, table.contiguous(), True)
         ctx.plan = plan
         ctx.save_for_backward(qkv, lam, saved)
         return out.view(out.shape[0], out.shape[1], -1)
@@ -254,16 +284,15 @@ class _GridSelfAttention(torch.autograd.Function):
     def backward(ctx, dout):
         qkv, lam, saved = ctx.saved_tensors
         plan = ctx.plan
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        dtable, dlam = _backward(plan, *_split_qkv(qkv, plan), saved, None if lam is None else lam.contiguous(), None, dout.reshape(plan.out_shape),
-                                 *_split_qkv(dqkv, plan), ctx.needs_input_grad[1])
+        dqkv = _like(qkv)
+        p = _describe_qkv(plan, qkv, lam)
+        p.line = saved.data_ptr()
+        g = AttentionGrads.from_buffer_copy(plan.grads_qkv)
+        at, step = dqkv.data_ptr(), plan.heads * plan.maps * plan.d * dqkv.element_size()
+        g.dq, g.dk, g.dv = at, at + step, at + 2 * step
+        dout = _dense16(dout)
+        dtable, dlam = _backward(plan, p, g, saved, dout, ctx.needs_input_grad[1])
         return dqkv, dtable, dlam, None
-
-
-def _split_qkv(t, plan):
-    c = t.shape[2] // 3
-    maps, h, d = plan.maps, plan.heads, plan.d
-    return tuple(t[..., i * c:(i + 1) * c].unflatten(2, (h * maps, d) if i < 2 else (h, d * maps)) for i in range(3))
 
 
 def _numbers(x):
@@ -271,7 +300,11 @@ def _numbers(x):
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, scale):
@@ -289,8 +322,8 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
         _parameter("lam", lam, (plan.heads,), dev)
     if lengths is not None:
         _on_gpu("lengths", lengths, dev)
-        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0],):
-            _fail(f"lengths: expected int32 [{q.shape[0]}], got {lengths.dtype} {list(lengths.shape)}")
+        if lengths.dtype != torch.int32 or lengths.shape != (plan.batch,):
+            _fail(f"lengths: expected int32 [{plan.batch}], got {lengths.dtype} {list(lengths.shape)}")
         lengths = lengths.contiguous()
     needs = _needs_grad(q, k, v, table, lam)
     if plan.desc is None:                                    # nothing is asked for
@@ -299,7 +332,8 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if needs:
         return _GridAttention.apply(q, k, v, table, lam, lengths, plan)
-    return _forward(plan, q, k, v, table.contiguous(), None if lam is None else lam.contiguous(), lengths, False)[0]
+    table, lam = table.contiguous(), None if lam is None else lam.contiguous()
+    return _forward(plan, _describe(plan, q, k, v, lengths, lam), q.dtype, dev, table, False)[0]
 
 
 def grid_attention(q, k, v, table, grid, max_distance=64, lengths=None, q_start=0, scale=None):
@@ -345,14 +379,14 @@ def grid_self_attention(qkv, heads, table, grid, lam=None, max_distance=64, scal
     d = c3 // (3 * heads * maps)
     shape, grid = (b, n, heads * maps, d), _numbers(grid)
     plan = _plan(maps, shape, shape, (b, n, heads, d * maps), qkv.dtype, table.shape, grid, _numbers(max_distance), 0, scale)
-    if n != int(grid[0]) * int(grid[1]):
+    if n != plan.grid[0] * plan.grid[1]:
         _fail(f"{n} tokens are not the grid {grid}")
     if plan.desc is None:
         return qkv[..., :c3 // 3]
     if _needs_grad(qkv, table, lam):
         return _GridSelfAttention.apply(qkv, table, lam, plan)
-    out = _forward(plan, *_split_qkv(_rows16(qkv), plan), table.contiguous(), None if lam is None else lam.contiguous(), None, False)[0]
-    return out.view(b, n, c3 // 3)
+    qkv, table, lam = _dense16(qkv), table.contiguous(), None if lam is None else lam.contiguous()
+    return _forward(plan, _describe_qkv(plan, qkv, lam), qkv.dtype, qkv.device, table, False)[0].view(b, n, c3 // 3)
 
 
 # ---------------------------------------------------------------------------------------------------------------------- norms
