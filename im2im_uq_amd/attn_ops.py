@@ -242,6 +242,12 @@ def _backward(plan, p, g, saved, dout, want_table):
     return dtable, dlam
 
 
+def _once(backward):
+    """once_differentiable, whose bookkeeping a first-order pass (no gradient mode in its backward) goes without"""
+    strict = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _GridAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, lam, lengths, plan):
@@ -253,7 +259,7 @@ class _GridAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dout):
         q, k, v, lam, lengths, saved = ctx.saved_tensors
         plan = ctx.plan
@@ -280,7 +286,7 @@ class _GridSelfAttention(torch.autograd.Function):
         return out.view(out.shape[0], out.shape[1], -1)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dout):
         qkv, lam, saved = ctx.saved_tensors
         plan = ctx.plan
@@ -444,7 +450,7 @@ class _NormGate(torch.autograd.Function):
         return (y, h) if f is not None and h is not None else h if f is None else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, *grads):
         s = ctx.s
         x, f, gate, *params = ctx.saved_tensors

@@ -301,6 +301,28 @@ def test_on_another_device():
     assert all(torch.equal(got[n].cpu(), want[n].cpu()) for n in want)
 
 
+@pytest.mark.parametrize("maps", [1, 2])
+def test_no_second_derivatives(maps):
+    """create_graph gives the same gradients and refuses to be differentiated again, rather than giving a gradient of nothing"""
+    grid = (5, 7)
+    o = operands(maps, F32, grid, 2, 2, 32, (4, 4))
+    names = [n for n in o if n != "dout" and o[n] is not None]
+    for n in names:
+        o[n] = o[n].detach().requires_grad_()
+    leaves = [o[n] for n in names]
+    plain = torch.autograd.grad(call(o, grid), leaves, o["dout"])
+    graph = torch.autograd.grad(call(o, grid), leaves, o["dout"], create_graph=True)
+    for a, b in zip(plain, graph):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        graph[0].sum().backward()
+    graph = torch.autograd.grad(call(o, grid), leaves, o["dout"].clone().requires_grad_(), create_graph=True)
+    for a, b in zip(plain, graph):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        graph[0].sum().backward()
+
+
 def test_nothing_asked_for():
     o = operands(1, F32, (2, 3), 2, 2, 8, (2, 2))
     t = o["q"][:0].requires_grad_(True)
