@@ -143,15 +143,15 @@ for _name, (_res, _args) in SIGNATURES.items():
 
 class AttentionDesc(ctypes.Structure):
     """im2im_attention_desc"""
-    _fields_ = [("q", _ptr), ("k", _ptr), ("v", _ptr), ("line", _ptr), ("lengths", _ptr), ("lam", _ptr), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3),
-                ("v_stride", _i64 * 3), ("B", _i32), ("Lq", _i32), ("Lk", _i32), ("H", _i32), ("D", _i32), ("maps", _i32), ("gh", _i32), ("gw", _i32),
-                ("q_start", _i32), ("dtype", _i32), ("scale", _f32)]
+    _fields_ = [("q", _ptr), ("k", _ptr), ("v", _ptr), ("line", _ptr), ("table", _ptr), ("thr_y", _ptr), ("thr_x", _ptr), ("lengths", _ptr), ("lam", _ptr),
+                ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("B", _i32), ("Lq", _i32), ("Lk", _i32), ("H", _i32), ("D", _i32), ("maps", _i32), ("gh", _i32), ("gw", _i32),
+                ("q_start", _i32), ("dtype", _i32), ("ny", _i32), ("nx", _i32), ("scale", _f32)]
 
 
 class AttentionGrads(ctypes.Structure):
     """im2im_attention_grads"""
     _fields_ = [("dout", _ptr), ("lse", _ptr), ("map_out", _ptr), ("dq", _ptr), ("dk", _ptr), ("dv", _ptr), ("dtable", _ptr), ("dlam", _ptr),
-                ("thr_y", _ptr), ("thr_x", _ptr), ("dq_stride", _i64 * 3), ("dk_stride", _i64 * 3), ("dv_stride", _i64 * 3), ("ny", _i32), ("nx", _i32)]
+                ("dq_stride", _i64 * 3), ("dk_stride", _i64 * 3), ("dv_stride", _i64 * 3)]
 
 
 class NormGateDesc(ctypes.Structure):

@@ -157,6 +157,8 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
     t = p.desc = AttentionDesc()
     t.B, t.Lq, t.Lk, t.H, t.D, t.maps, t.gh, t.gw, t.q_start, t.dtype, t.scale = b, lq, lk, heads, d, maps, gh, gw, q_start, _DT[dtype], scale
     t.q = t.k = t.v = t.line = t.lam = 16
+    t.ny, t.nx = table_shape[:2]
+    t.thr_y, t.thr_x = (ctypes.cast(x, ctypes.c_void_p) for x in p.thr)
     c = heads * maps * d
     t.q_stride[:], t.k_stride[:], t.v_stride[:] = (lq * c, c, d), (lk * c, c, d), (lk * c, c, d * maps)
     p.fwd_ws = lib.im2im_attention_fwd_workspace_bytes(ctypes.byref(t))
@@ -165,8 +167,6 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
         check(-1, "im2im_attention_fwd")
     g = p.grads = AttentionGrads()
     g.dq_stride[:], g.dk_stride[:], g.dv_stride[:] = t.q_stride, t.k_stride, t.v_stride
-    g.ny, g.nx = table_shape[:2]
-    g.thr_y, g.thr_x = (ctypes.cast(x, ctypes.c_void_p) for x in p.thr)
     # the same for q, k and v side by side in one tensor
     p.desc_qkv, p.grads_qkv = AttentionDesc.from_buffer_copy(t), AttentionGrads.from_buffer_copy(g)
     for x in (p.desc_qkv.q_stride, p.desc_qkv.k_stride, p.grads_qkv.dq_stride, p.grads_qkv.dk_stride):
@@ -203,12 +203,16 @@ def _describe_qkv(plan, qkv, lam):
 def _forward(plan, p, dtype, dev, table, keep):
     """(out, saved) for the description `p` (its line is filled in): `saved` holds the line, log-sums and map results"""
     out = torch.empty(plan.out_shape, dtype=dtype, device=dev)
-    saved = torch.empty(plan.save if keep else plan.lse_at, dtype=torch.uint8, device=dev)
     ws = torch.empty(plan.fwd_ws, dtype=torch.uint8, device=dev) if plan.fwd_ws else None
-    p.line = line = saved.data_ptr()
     guard = _guard(dev)
     try:
         stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        if not keep and plan.out_shape[1] == 1:              # one query: its bias comes from the table itself
+            p.line, p.table = None, table.data_ptr()
+            check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), None, None, _ptr(ws), plan.fwd_ws, stream), "im2im_attention_fwd")
+            return out, None
+        saved = torch.empty(plan.save if keep else plan.lse_at, dtype=torch.uint8, device=dev)
+        p.line = line = saved.data_ptr()
         ny, nx, heads = plan.table_shape
         check(lib.im2im_relpos_line(table.data_ptr(), ny, nx, heads, plan.thr[0], plan.thr[1], plan.grid[0], plan.grid[1], line, stream), "im2im_relpos_line")
         check(lib.im2im_attention_fwd(ctypes.byref(p), out.data_ptr(), line + plan.lse_at if keep else None, line + plan.map_at if keep else None,

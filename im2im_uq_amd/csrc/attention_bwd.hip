@@ -631,8 +631,7 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
     for (int x = 0; x < 3; ++x) IM2IM_REQUIRE(stride[t][x] > 0 && (stride[t][x] * e) % 16 == 0);
   }
   const bool table = g->dtable != nullptr;
-  IM2IM_REQUIRE(!table || (g->ny >= 1 && g->ny <= 64 && (g->ny == 1 || g->ny % 2 == 0) && g->nx >= 1 && g->nx <= 64 && (g->nx == 1 || g->nx % 2 == 0)));
-  IM2IM_REQUIRE(!table || ((g->ny <= 2 || g->thr_y) && (g->nx <= 2 || g->thr_x)));
+  IM2IM_REQUIRE(p->line && (!table || attn_buckets_ok(p->ny, p->nx, p->thr_y, p->thr_x)));
   IM2IM_REQUIRE((int64_t)a.H * a.dv * e * KEYS < (1ll << 31));
   set_tiles(&a);
   const BwdLayout l = set_groups(&a, p->maps, table, ws_bytes);
@@ -659,9 +658,9 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   BucketArgs s = {};
   s.line = table ? line : nullptr;
   s.dlam_part = a.dlam_part; s.dtable = g->dtable; s.dlam = g->dlam;
-  s.ny = table ? g->ny : 0; s.nx = table ? g->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.nq;
-  for (int m = 0; m + 1 < s.ny / 2; ++m) s.thr_y[m] = g->thr_y[m];
-  for (int m = 0; m + 1 < s.nx / 2; ++m) s.thr_x[m] = g->thr_x[m];
+  s.ny = table ? p->ny : 0; s.nx = table ? p->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.nq;
+  for (int m = 0; m + 1 < s.ny / 2; ++m) s.thr_y[m] = p->thr_y[m];
+  for (int m = 0; m + 1 < s.nx / 2; ++m) s.thr_x[m] = p->thr_x[m];
   hipLaunchKernelGGL(attn_bucket_sum_kernel, dim3((unsigned)(s.ny * s.nx + (p->maps == 2)), (unsigned)a.H), dim3(64), 0, st, s);
   return check_launch("attn_bucket_sum_kernel");
 }

@@ -21,6 +21,8 @@ struct AttnArgs {
   const void *q, *k, *v;
   int64_t qs[3], ks[3], vs[3];        // element strides: batch, token, head
   const float* line;                  // [H][line_len], in units of log2
+  const float* table;                 // [ny][nx][H]: a single query's bias, when there is no line
+  int ny, nx, thr[64];                // smallest distance of bucket 1, 2, ...: down from 0 on, across from 32 on
   const int32_t* lengths;             // [B] or null
   const float* lam;                   // [H] (two maps)
   int B, Lq, Lk, H, d, dv, gw, line_len, line_off, q_start, nq, nk;
@@ -227,6 +229,26 @@ __device__ __forceinline__ void fetch_window(float* to, const float* line, int l
   for (int w = wave_index() * 64; w < n; w += 64 * WAVES) load4_to_lds(line + max(0, min(first + w + lane, line_len - 1)), to + w);
 }
 
+// bucket of a signed distance; `thr`: lane `from` + m holds the smallest distance of bucket m + 1, searched by halves (all lanes take part)
+__device__ __forceinline__ int lane_bucket(int delta, int n, int thr, int from) {
+  if (n == 1) return 0;
+  const int side = n / 2, t = delta < 0 ? -delta : delta;
+  int b = 0;
+#pragma unroll
+  for (int step = 16; step >= 1; step >>= 1) {
+    if (step >= side) continue;
+    const int bound = __shfl(thr, from + b + step - 1);
+    if (b + step < side && t >= bound) b += step;
+  }
+  return delta > 0 ? b + side : b;
+}
+
+// a table's entry in units of log2.  A finite entry stays finite (the type's lowest value is a large bias; -infinity is a mask).
+__device__ __forceinline__ float bias_log2(float t) {
+  const float v = t * LOG2E;
+  return v == -INFINITY && t != -INFINITY ? -1.7e38f : v;
+}
+
 // LDS buffers of tiles: two (the next tile's loads run behind this tile's work, one barrier a tile), one for the widest heads in 32 bits
 template <typename T> __host__ __device__ constexpr int buffers(int elements) { return elements * (int)sizeof(T) <= 512 ? 2 : 1; }
 template <typename T> __host__ __device__ constexpr size_t tile_bytes(int elements) { return (size_t)KEYS * elements * sizeof(T); }
@@ -268,6 +290,7 @@ inline int code_span(int64_t n, int gh, int gw) { return (int)(gh == 1 ? n - 1 :
 inline int window_floats(int gh, int gw) { return code_span(ROWS, gh, gw) + code_span(KEYS, gh, gw) + 1; }
 inline int round64(int n) { return (n + 63) / 64 * 64; }
 
+bool attn_buckets_ok(int32_t ny, int32_t nx, const int32_t* thr_y, const int32_t* thr_x);
 int attn_check(const im2im_attention_desc* p, AttnArgs* a);      // validates the description, fills the common fields
 int attn_allow_lds(const void* kernel, size_t bytes);            // raises the kernel's dynamic LDS limit on the current device
 

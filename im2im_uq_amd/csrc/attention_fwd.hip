@@ -32,11 +32,7 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
   if (idx >= a.len) return;
   const int w = 2 * a.gw - 1;
   const int b = axis_bucket(idx / w - (a.gh - 1), a.ny, a.thr_y) * a.nx + axis_bucket(idx % w - (a.gw - 1), a.nx, a.thr_x);
-  const float t = a.table[(int64_t)b * a.H + h];
-  // a finite entry stays finite in units of log2 (the type's lowest value is a large bias; -infinity is a mask)
-  float v = t * LOG2E;
-  if (v == -INFINITY && t != -INFINITY) v = -1.7e38f;
-  a.line[(int64_t)h * a.len + idx] = v;
+  a.line[(int64_t)h * a.len + idx] = bias_log2(a.table[(int64_t)b * a.H + h]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- forward
@@ -51,7 +47,8 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // for 168 at 16 x 40x40 x 4 x 64).
 constexpr float GROW = 8.f;
 
-template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS>
+// TOKEN (one query, nothing saved): a key's bias is taken from the table itself, a launch and the line less; a tile's window is its keys in their order.
+template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS, bool TOKEN = false>
 __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
@@ -91,7 +88,8 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
   const int t0 = sp * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, (len + KEYS - 1) / KEYS);
   const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)(MAPS * h) * a.ks[2];
   const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
-  const float* line = a.line + (int64_t)h * a.line_len;
+  const float* line = TOKEN ? a.table + h : a.line + (int64_t)h * a.line_len;
+  const int thr = TOKEN ? a.thr[lane] : 0, q_row = TOKEN ? a.q_start / a.gw : 0, q_col = TOKEN ? a.q_start % a.gw : 0;
 
   TileFetch<T, DQ> kt;
   TileFetch<T, DV> vt;
@@ -99,7 +97,17 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
   vt.prepare(a.vs[1]);
   const bool full = a.d == DQ && a.dv == DV;
   Raster keys(t0 * KEYS, a.gw);
+  // TOKEN: a wave without a query looks up its lanes' keys of the coming tile (behind the last one: any entry) while the others work on this one
+  const bool spare = TOKEN && wave_index() == WAVES - 1;
+  auto entry = [&] { return line[(int64_t)(lane_bucket(keys.row - q_row, a.ny, thr, 0) * a.nx + lane_bucket(keys.col - q_col, a.nx, thr, 32)) * a.H]; };
+  float ahead = spare ? entry() : 0.f;
   auto fetch = [&](int t, char* to) {                             // tiles in their order
+    if (spare) {
+      int* codes = reinterpret_cast<int*>(to + TILES);
+      reinterpret_cast<float*>(codes + KEYS)[lane] = bias_log2(ahead);
+      codes[lane] = 4 * lane;
+      keys.next();
+    }
     const int j0 = t * KEYS, valid = min(len - j0, KEYS);
     const T *k = kp + (int64_t)j0 * a.ks[1], *v = vp + (int64_t)j0 * a.vs[1];
     if (full && valid == KEYS) {
@@ -110,6 +118,10 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) kt.part(to + m * KT, k + m * a.ks[2], a.ks[1], valid, a.d);
       vt.part(to + MAPS * KT, v, a.vs[1], valid, a.dv);
+    }
+    if (TOKEN) {
+      if (spare) ahead = entry();
+      return;
     }
     const int code = keys.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
     keys.next();
@@ -378,9 +390,14 @@ int attn_allow_lds(const void* kernel, size_t bytes) {
   return IM2IM_OK;
 }
 
+bool attn_buckets_ok(int32_t ny, int32_t nx, const int32_t* thr_y, const int32_t* thr_x) {
+  return ny >= 1 && ny <= 64 && (ny == 1 || ny % 2 == 0) && nx >= 1 && nx <= 64 && (nx == 1 || nx % 2 == 0) && (ny <= 2 || thr_y) && (nx <= 2 || thr_x);
+}
+
 int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   IM2IM_REQUIRE(p != nullptr);
-  IM2IM_REQUIRE(p->q && p->k && p->v && p->line);
+  IM2IM_REQUIRE(p->q && p->k && p->v);
+  IM2IM_REQUIRE(p->line || (p->Lq == 1 && p->table && attn_buckets_ok(p->ny, p->nx, p->thr_y, p->thr_x)));
   IM2IM_REQUIRE(p->dtype == IM2IM_F32 || p->dtype == IM2IM_BF16);
   IM2IM_REQUIRE(p->maps == 1 || p->maps == 2);
   IM2IM_REQUIRE(p->maps == 1 || p->lam != nullptr);
@@ -416,9 +433,10 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   return IM2IM_OK;
 }
 
-// Half as many queries for each workgroup where there would be fewer than two workgroups a CU (23 -> 21 us for 320 of them: 10 x 20x20 x 8 x 64)
+// Half as many queries for each workgroup where there would be fewer than two workgroups a CU (23 -> 21 us for 320 of them: 10 x 20x20 x 8 x 64),
+// or one query has the workgroup for itself
 static void set_queries(AttnArgs* a) {
-  a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 512 ? 2 : 1;
+  a->ks_q = a->Lq == 1 || (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 512 ? 2 : 1;
   a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);
 }
 
@@ -434,6 +452,8 @@ static int key_splits(const AttnArgs& a) {
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
   auto kern = a.ks_q == 2 ? attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, ROW4, 2> : attn_fwd_kernel<T, DQ, DV, MAPS, SAVE, ROW4, 1>;
+  if constexpr (!SAVE && ROW4)
+    if (!a.line) kern = attn_fwd_kernel<T, DQ, DV, MAPS, false, true, 2, true>;
   size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4);
   if (a.ks_q == 2) smem = std::max<size_t>(smem, 2 * MAPS * (DV / 2 + 2) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
@@ -449,7 +469,7 @@ template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4> static int
 }
 
 template <typename T, int DQ, int DV, int MAPS, bool SAVE> static int launch_fwd(const AttnArgs& a, hipStream_t st) {
-  return a.row4 ? launch_fwd<T, DQ, DV, MAPS, SAVE, true>(a, st) : launch_fwd<T, DQ, DV, MAPS, SAVE, false>(a, st);
+  return a.row4 || !a.line ? launch_fwd<T, DQ, DV, MAPS, SAVE, true>(a, st) : launch_fwd<T, DQ, DV, MAPS, SAVE, false>(a, st);
 }
 
 template <typename T, bool SAVE> static int dispatch_fwd(const AttnArgs& a, int maps, hipStream_t st) {
@@ -471,9 +491,8 @@ extern "C" int64_t im2im_relpos_line_len(int32_t gh, int32_t gw) {
 extern "C" int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, const int32_t* thr_y, const int32_t* thr_x, int32_t gh,
                                  int32_t gw, float* line, im2im_stream_t stream) {
   IM2IM_REQUIRE(table && line && H >= 1 && H <= 65535);
-  IM2IM_REQUIRE(ny >= 1 && ny <= 64 && (ny == 1 || ny % 2 == 0) && nx >= 1 && nx <= 64 && (nx == 1 || nx % 2 == 0));
+  IM2IM_REQUIRE(attn_buckets_ok(ny, nx, thr_y, thr_x));
   IM2IM_REQUIRE(gh >= 1 && gw >= 1 && (int64_t)gh * gw <= (1 << 24));
-  IM2IM_REQUIRE((ny <= 2 || thr_y) && (nx <= 2 || thr_x));
   LineArgs a = {};
   a.table = table; a.line = line; a.ny = ny; a.nx = nx; a.H = H; a.gh = gh; a.gw = gw; a.len = (2 * gh - 1) * (2 * gw - 1);
   for (int m = 0; m + 1 < ny / 2; ++m) a.thr_y[m] = thr_y[m];
@@ -495,7 +514,13 @@ extern "C" int im2im_attention_fwd(const im2im_attention_desc* p, void* out, flo
   AttnArgs a = {};
   if (int rc = attn_check(p, &a)) return rc;
   IM2IM_REQUIRE(out && (lse != nullptr) == (map_out != nullptr));
+  IM2IM_REQUIRE(p->line || !lse);
   a.out = out; a.lse = lse; a.osave = map_out;
+  if (!p->line) {
+    a.table = p->table; a.ny = p->ny; a.nx = p->nx; a.window = KEYS;
+    for (int m = 0; m + 1 < p->ny / 2; ++m) a.thr[m] = p->thr_y[m];
+    for (int m = 0; m + 1 < p->nx / 2; ++m) a.thr[32 + m] = p->thr_x[m];
+  }
   set_queries(&a);
   a.splits = key_splits(a);
   a.tiles_per_split = (int)cdiv(cdiv(a.Lk, KEYS), a.splits);

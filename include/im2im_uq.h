@@ -582,6 +582,8 @@ int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, con
  *   The queries are the grid's tokens q_start .. q_start + Lq - 1, the keys its tokens 0 .. Lk - 1 (gw <= 512 unless gh == 1).
  *   lengths: device int32 [B] or null (all Lk), clipped to 0..Lk; keys behind it take no part, whatever they hold; a row without
  *   keys gives zeros (and zero gradients).  A table entry of -infinity masks its pairs.
+ *   line: of im2im_relpos_line.  ny, nx, thr_y, thr_x: the table's; the backward needs them for dtable.  A forward of one query (Lq = 1) that saves
+ *   nothing may have line = null and table instead: it takes each key's bias from there.
  *   lse / map_out (both or neither): saved for the backward: lse [B*H][maps][Lq] fp32, map_out [B*H][Lq][maps][D*maps] fp32.
  * im2im_attention_bwd: dout [B][Lq][H][D*maps] dense; dq / dk / dv in the types and index order of q / k / v with their own strides; dtable
  *   [ny][nx][H] fp32 or null; dlam [H] fp32 (maps = 2).  Every sum has a fixed order: repeated calls with the same workspace size give the same
@@ -590,10 +592,12 @@ int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, con
 typedef struct {
   const void *q, *k, *v;
   const float* line;
+  const float* table;
+  const int32_t *thr_y, *thr_x;
   const int32_t* lengths;
   const float* lam;
   int64_t q_stride[3], k_stride[3], v_stride[3];
-  int32_t B, Lq, Lk, H, D, maps, gh, gw, q_start, dtype;
+  int32_t B, Lq, Lk, H, D, maps, gh, gw, q_start, dtype, ny, nx;
   float scale;
 } im2im_attention_desc;
 typedef struct {
@@ -601,9 +605,7 @@ typedef struct {
   const float *lse, *map_out;
   void *dq, *dk, *dv;
   float *dtable, *dlam;
-  const int32_t *thr_y, *thr_x;
   int64_t dq_stride[3], dk_stride[3], dv_stride[3];
-  int32_t ny, nx;
 } im2im_attention_grads;
 int64_t im2im_attention_fwd_workspace_bytes(const im2im_attention_desc* p);
 int im2im_attention_fwd(const im2im_attention_desc* p, void* out, float* lse, float* map_out, void* ws, int64_t ws_bytes,

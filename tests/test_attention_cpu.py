@@ -41,7 +41,7 @@ def test_cpu_tensors_are_refused():
 
 def desc(**kw):
     p = AttentionDesc()
-    base = dict(q=4096, k=4096, v=4096, line=4096, B=2, Lq=6, Lk=6, H=2, D=16, maps=1, gh=2, gw=3, q_start=0, dtype=0, scale=0.25)
+    base = dict(q=4096, k=4096, v=4096, line=4096, B=2, Lq=6, Lk=6, H=2, D=16, maps=1, gh=2, gw=3, q_start=0, dtype=0, ny=2, nx=2, scale=0.25)
     for k, v in {**base, **kw}.items():
         setattr(p, k, v)
     for s in (p.q_stride, p.k_stride, p.v_stride):
@@ -68,6 +68,12 @@ def test_attention_entry_refusals():
     assert need > 0
     assert lib.im2im_attention_fwd(N(long_), 4096, None, None, None, 0, None) == -1               # no workspace
     assert lib.im2im_attention_fwd(N(long_), 4096, None, None, 4096, need - 1, None) == -1
+    token = dict(Lq=1, line=0, table=4096)                                                         # one query, its bias from the table
+    assert lib.im2im_attention_fwd_workspace_bytes(N(desc(**token))) == 0
+    for kw in (dict(table=0), dict(Lq=2), dict(ny=0), dict(nx=3), dict(ny=66), dict(nx=8)):
+        assert lib.im2im_attention_fwd(N(desc(**{**token, **kw})), 4096, None, None, None, 0, None) == -1, kw
+    assert lib.im2im_attention_fwd(N(desc(**token)), 4096, 4096, 4096, None, 0, None) == -1       # nothing to save
+    assert lib.im2im_attention_bwd(N(desc(**token)), N(AttentionGrads()), 4096, 1 << 30, None) == -1
     g = AttentionGrads()
     for name in ("dout", "lse", "map_out", "dq", "dk", "dv", "dtable"):
         setattr(g, name, 4096)
@@ -75,11 +81,8 @@ def test_attention_entry_refusals():
         s[:] = (192, 32, 16)
     need = lib.im2im_attention_bwd_workspace_bytes(N(desc()), 1)
     for n in (0, 3, 66):
-        g.ny, g.nx = n, 2
-        assert lib.im2im_attention_bwd(N(desc()), N(g), 4096, need, None) == -1
-    g.ny, g.nx = 8, 2                                                                             # no borders
-    assert lib.im2im_attention_bwd(N(desc()), N(g), 4096, need, None) == -1
-    g.ny = 2
+        assert lib.im2im_attention_bwd(N(desc(ny=n)), N(g), 4096, need, None) == -1
+    assert lib.im2im_attention_bwd(N(desc(ny=8)), N(g), 4096, need, None) == -1                   # no borders
     assert lib.im2im_attention_bwd(N(desc()), N(g), 4096, 512, None) == -1                        # not enough for one image at a time either
     assert lib.im2im_attention_bwd(N(desc()), N(g), None, need, None) == -1
     assert lib.im2im_attention_bwd(N(desc(maps=2, lam=4096)), N(g), 4096, 1 << 30, None) == -1    # no dlam

@@ -154,6 +154,23 @@ def test_few_queries(maps, dtype, grid, lq, q_start, lk):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,d,heads,b,grid,buckets", [
+    (1, 64, 2, 2, (5, 7), (4, 6)), (1, 40, 1, 1, (1, 1), (1, 1)), (1, 32, 8, 64, (9, 15), (64, 64)), (1, 128, 2, 1, (130, 1), (32, 1)),
+    (1, 24, 3, 1, (1, 300), (1, 64)), (2, 32, 2, 2, (5, 7), (6, 4)), (2, 64, 1, 2, (17, 33), (16, 8)), (2, 16, 9, 57, (2, 65), (2, 2))])
+def test_single_token(maps, d, heads, b, grid, buckets, dtype):
+    """one query at the grid's ends and inside, with lengths that leave no key, one key and half a tile, and masks in its table"""
+    n = grid[0] * grid[1]
+    for at in sorted({0, n // 3, n - 1}):
+        o = operands(maps, dtype, grid, b, heads, d, buckets, lq=1, seed=at)
+        o["table"][0, 0, 0], o["table"][-1, -1, -1] = -math.inf, torch.finfo(F32).min
+        lengths = torch.tensor([(n, 0, 1, 33)[x % 4] for x in range(b)], dtype=torch.int32, device=DEV)
+        check({"out": call(o, grid, q_start=at, lengths=lengths)}, reference(o, grid, False, q_start=at, lengths=lengths))
+        whole = operands(maps, dtype, grid, b, heads, d, buckets, seed=at)
+        alone = call({**o, "q": whole["q"][:, at:at + 1]}, grid, q_start=at)
+        check({"out": alone}, reference({**o, "q": whole["q"][:, at:at + 1]}, grid, False, q_start=at))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("maps", [1, 2])
 def test_table_masks(maps, dtype):
     """entries of -infinity mask their pairs, a row of the grid loses all its keys to them; the type's lowest value is a bias like others"""
