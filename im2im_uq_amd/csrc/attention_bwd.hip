@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   double* ring = reinterpret_cast<double*>(smem + NBUF * buffer);          // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
   __shared__ float red[WAVES];
 
-  const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, gh_ = lin / a.nq, h = gh_ % a.H, group = gh_ / a.H;
+  const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, h = lin / a.nq / a.groups, group = lin / a.nq % a.groups;
   const int slot = group * a.nq + qt;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   if (threadIdx.x < 4 * NBUF)
     *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
-  const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, bh = lin / a.nk, h = bh % a.H, b = bh / a.H;
+  const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, h = lin / a.nk / a.B, b = lin / a.nk % a.B, bh = b * a.H + h;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
   const int k0 = kt * QR, k_last = min(k0 + QR, a.Lk) - 1;

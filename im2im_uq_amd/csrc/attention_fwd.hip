@@ -59,7 +59,8 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
   const size_t buffer = TILES + KEYS * 4 + (size_t)a.window * 4;           // tiles, codes, window
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.splits, item = lin / a.splits;
-  const int qt = item % a.nq, bh = item / a.nq, h = bh % a.H, b = bh / a.H;
+  // all images of a head, then the next head: each XCD gets many images, whose lengths may differ (224 -> 215 us at 16 x 40x40 x 4 x 2 x 64, half to full)
+  const int qt = item % a.nq, h = item / a.nq / a.B, b = item / a.nq % a.B, bh = b * a.H + h;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31);
