@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 
 import torch
 
@@ -117,7 +118,7 @@ class _Plan:
 
 
 @functools.lru_cache(maxsize=1024)
-def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distance, q_start, scale):
+def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distance, scale):
     if dtype not in _DT:
         _fail(f"q, k, v: fp32 or bf16, got {dtype}")
     if not len(q_shape) == len(k_shape) == len(v_shape) == 4:
@@ -138,8 +139,8 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
         _fail(f"grid {grid}: at least 1 x 1, at most 2**24 tokens, and at most {MAX_GRID_WIDTH} wide unless it is one row")
     if lk > gh * gw:
         _fail(f"{lk} keys do not fit the grid {grid}")
-    if q_start < 0 or q_start + lq > gh * gw:
-        _fail(f"queries {q_start} .. {q_start + lq - 1} are not tokens of the grid {grid}")
+    if lq > gh * gw:
+        _fail(f"{lq} queries are not tokens of the grid {grid}")
     if len(table_shape) != 3 or table_shape[2] != heads:
         _fail(f"table: expected fp32 [vertical buckets, horizontal buckets, {heads}], got {list(table_shape)}")
     p = _Plan()
@@ -155,7 +156,7 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
         return p
     # the description of dense operands with the pointers left open, and the sizes that follow from it
     t = p.desc = AttentionDesc()
-    t.B, t.Lq, t.Lk, t.H, t.D, t.maps, t.gh, t.gw, t.q_start, t.dtype, t.scale = b, lq, lk, heads, d, maps, gh, gw, q_start, _DT[dtype], scale
+    t.B, t.Lq, t.Lk, t.H, t.D, t.maps, t.gh, t.gw, t.dtype, t.scale = b, lq, lk, heads, d, maps, gh, gw, _DT[dtype], scale
     t.q = t.k = t.v = t.line = t.lam = 16
     t.ny, t.nx = table_shape[:2]
     t.thr_y, t.thr_x = (ctypes.cast(x, ctypes.c_void_p) for x in p.thr)
@@ -181,8 +182,9 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
     return p
 
 
-def _describe(plan, q, k, v, lengths, lam):
+def _describe(plan, q, k, v, lengths, lam, q_start):
     p = AttentionDesc.from_buffer_copy(plan.desc)
+    p.q_start = q_start
     p.q, p.k, p.v, p.lengths, p.lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), _ptr(lam)
     if not q.is_contiguous():
         p.q_stride[:] = q.stride()[:3]
@@ -254,11 +256,11 @@ def _once(backward):
 
 class _GridAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, lam, lengths, plan):
+    def forward(ctx, q, k, v, table, lam, lengths, plan, q_start):
         lam = None if lam is None else lam.contiguous()
-        p = _describe(plan, q, k, v, lengths, lam)
+        p = _describe(plan, q, k, v, lengths, lam, q_start)
         out, saved = _forward(plan, p, q.dtype, q.device, table.contiguous(), True)
-        ctx.plan = plan
+        ctx.plan, ctx.q_start = plan, q_start
         ctx.save_for_backward(q, k, v, lam, lengths, saved)
         return out
 
@@ -268,13 +270,13 @@ class _GridAttention(torch.autograd.Function):
         q, k, v, lam, lengths, saved = ctx.saved_tensors
         plan = ctx.plan
         dq, dk, dv = _like(q), _like(k), _like(v)
-        p = _describe(plan, q, k, v, lengths, lam)
+        p = _describe(plan, q, k, v, lengths, lam, ctx.q_start)
         p.line = saved.data_ptr()
         g = AttentionGrads.from_buffer_copy(plan.grads)
         g.dq, g.dk, g.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         dout = _dense16(dout)
         dtable, dlam = _backward(plan, p, g, saved, dout, ctx.needs_input_grad[3])
-        return dq, dk, dv, dtable, dlam, None, None
+        return dq, dk, dv, dtable, dlam, None, None, None
 
 
 class _GridSelfAttention(torch.autograd.Function):
@@ -305,8 +307,25 @@ class _GridSelfAttention(torch.autograd.Function):
         return dqkv, dtable, dlam, None
 
 
-def _numbers(x):
-    return tuple(x) if isinstance(x, list) else x
+def _integers(name, x):
+    """`x`, a number or a pair of them, as plain ints: nothing that could change enters a plan's key"""
+    if type(x) is int or (type(x) is tuple and len(x) == 2 and type(x[0]) is int and type(x[1]) is int):
+        return x
+    try:
+        return tuple(operator.index(n) for n in x) if isinstance(x, (tuple, list)) else operator.index(x)
+    except (TypeError, RuntimeError):
+        _fail(f"{name}: expected whole numbers, got {x!r}")
+
+
+def _number(name, x):
+    if x is None or type(x) is float:
+        return x
+    if isinstance(x, torch.Tensor):
+        _fail(f"{name}: expected a number, got a tensor")
+    try:
+        return float(x)
+    except (TypeError, ValueError):
+        _fail(f"{name}: expected a number, got {x!r}")
 
 
 def _needs_grad(*tensors):
@@ -327,7 +346,12 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
         _fail(f"q, k, v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     if table.dtype != F32:
         _fail(f"table: expected fp32, got {table.dtype}")
-    plan = _plan(maps, q.shape, k.shape, v.shape, q.dtype, table.shape, _numbers(grid), _numbers(max_distance), q_start, scale)
+    plan = _plan(maps, q.shape, k.shape, v.shape, q.dtype, table.shape, _integers("grid", grid), _integers("max_distance", max_distance),
+                 _number("scale", scale))
+    q_start = _integers("q_start", q_start)                  # no part of the plan: token after token has another one
+    (gh, gw), lq = plan.grid, plan.out_shape[1]
+    if isinstance(q_start, tuple) or not 0 <= q_start <= gh * gw - lq:
+        _fail(f"q_start = {q_start}: {lq} queries from there on are not tokens of the grid {grid}")
     if maps == 2:
         _parameter("lam", lam, (plan.heads,), dev)
     if lengths is not None:
@@ -341,9 +365,9 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
         return out + 0 * q.sum() if needs else out
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if needs:
-        return _GridAttention.apply(q, k, v, table, lam, lengths, plan)
+        return _GridAttention.apply(q, k, v, table, lam, lengths, plan, q_start)
     table, lam = table.contiguous(), None if lam is None else lam.contiguous()
-    return _forward(plan, _describe(plan, q, k, v, lengths, lam), q.dtype, dev, table, False)[0]
+    return _forward(plan, _describe(plan, q, k, v, lengths, lam, q_start), q.dtype, dev, table, False)[0]
 
 
 def grid_attention(q, k, v, table, grid, max_distance=64, lengths=None, q_start=0, scale=None):
@@ -387,8 +411,8 @@ def grid_self_attention(qkv, heads, table, grid, lam=None, max_distance=64, scal
         _parameter("lam", lam, (heads,), qkv.device)
     b, n, c3 = qkv.shape
     d = c3 // (3 * heads * maps)
-    shape, grid = (b, n, heads * maps, d), _numbers(grid)
-    plan = _plan(maps, shape, shape, (b, n, heads, d * maps), qkv.dtype, table.shape, grid, _numbers(max_distance), 0, scale)
+    shape, grid = (b, n, heads * maps, d), _integers("grid", grid)
+    plan = _plan(maps, shape, shape, (b, n, heads, d * maps), qkv.dtype, table.shape, grid, _integers("max_distance", max_distance), _number("scale", scale))
     if n != plan.grid[0] * plan.grid[1]:
         _fail(f"{n} tokens are not the grid {grid}")
     if plan.desc is None:

@@ -53,7 +53,10 @@ template <int N> __device__ __forceinline__ void join_halves(f32x16* acc, float*
 // same key, so their places differ; the other 32 lanes have another key and add to a copy of their own; each wave has its own pair
 // of copies and its additions are in program order: no order is left open.  A copy is a ring over the line's index: the places
 // that the following tiles cannot reach any more are summed over the copies and written, each once.  The copies are 64-bit:
-// ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 3xx us at 78 images of 20 x 20, 8 x 64.
+// ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 226 us at 78 x 20x20 x 8 x 64.  ROW4: four
+// queries' terms of a diagonal are summed from lane to lane first; with that and the tiles' asynchronous loads 226 -> 152 us.
+// Bound by the latency of a wave's own chain (scores, probabilities, dP, dS, diagonals) at two waves a SIMD, which is what the registers allow: there the
+// vector unit issues in 36 % of the cycles, LDS is active in 29 %.  8 x 32x32 x 8 x 128: 125 us.
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
@@ -288,7 +291,9 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 }
 
 // ---------------------------------------------------------------------------------------------- keys' and values' gradients
-// One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.
+// One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.  Scores and dP are computed
+// once more (two of its four products): cheaper than writing and reading them.  78 x 20x20 x 8 x 64: 110 us, 465 TFLOP/s with them; at three workgroups a
+// CU it spills and loses what the third gains.
 template <typename T, int DQ, int DV, int MAPS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
@@ -473,7 +478,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
 
 // ------------------------------------------------------------------------------------------------------ joining the parts
 // line[h][x] = sum over the slots whose queries reach x: 64 places a workgroup, the slots dealt to its 16 waves (bound by the latency of these loads:
-// with four waves 28 us for 312 slots of 8 x 1521)
+// 10 us for 312 slots of 8 x 1521; with four waves 28)
 __global__ __launch_bounds__(1024) void attn_line_sum_kernel(const AttnArgs a, double* sum) {
   __shared__ double part[16][64];
   const int l = threadIdx.x & 63, x = blockIdx.x * 64 + l, h = blockIdx.y, wave = threadIdx.x >> 6;
@@ -540,7 +545,7 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 
 static void set_tiles(AttnArgs* a) {
   // half as many queries (keys) for each workgroup where there would be less than one workgroup a CU (fp32, 3 x 17x23 x 5 x 40: 66 -> 46 and
-  // 69 -> 44 us with 60 of them; with 320, 10 x 20x20 x 8 x 64 bf16, it costs: 39 -> 51 and 26 -> 27 us)
+  // 69 -> 44 us with 60 of them, 39 and 44 by now; with 320, 10 x 20x20 x 8 x 64 bf16, it costs: 39 -> 51 and 26 -> 27 us)
   a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 256 ? 2 : 1;
   a->ks_k = (int64_t)a->B * a->H * cdiv(a->Lk, ROWS) < 256 ? 2 : 1;
   a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);

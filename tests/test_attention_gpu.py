@@ -318,6 +318,19 @@ def test_on_another_device():
     assert all(torch.equal(got[n].cpu(), want[n].cpu()) for n in want)
 
 
+def test_numbers_of_other_kinds():
+    """numpy's and torch's whole numbers and lists are taken as they are at the call, whatever becomes of them later"""
+    import numpy as np
+    grid = (6, 7)
+    o = operands(1, F32, grid, 1, 1, 16, (4, 4), lq=1)
+    at = torch.tensor(3)
+    for t in (3, 11, 40):
+        at.fill_(t)
+        want = call(o, grid, q_start=t, max_distance=16, scale=0.5)
+        assert torch.equal(call(o, [np.int64(6), np.int32(7)], q_start=at, max_distance=[16, np.int16(16)], scale=np.float32(0.5)), want)
+        check({"out": want}, reference(o, grid, False, q_start=t, max_distance=16, scale=0.5))
+
+
 @pytest.mark.parametrize("maps", [1, 2])
 def test_no_second_derivatives(maps):
     """create_graph gives the same gradients and refuses to be differentiated again, rather than giving a gradient of nothing"""
@@ -382,6 +395,13 @@ def test_refusals():
     refused("grid", where=(0, 5))
     refused("grid", where=(2, 513))
     refused("grid =", where=20)
+    refused("whole numbers", where=(4.0, 5))
+    refused("whole numbers", q_start=0.5)
+    refused("whole numbers", q_start=None)
+    refused("not tokens", q_start=(0, 1))
+    refused("whole numbers", max_distance="far")
+    refused("a tensor", scale=torch.tensor(0.5))
+    refused("a number", scale="one")
     refused("lengths", lengths=torch.zeros(2, dtype=torch.int64, device=DEV))
     refused("lengths", lengths=torch.zeros(3, dtype=torch.int32, device=DEV))
     refused("GPU", lengths=torch.zeros(2, dtype=torch.int32))
