@@ -70,7 +70,13 @@ def _on_gpu(name, t, device=None):
         _fail(f"{name} is on {t.device}, the other operands on {device}")
 
 
+def _is(t, dtype, shape, device):
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
+
+
 def _parameter(name, t, shape, device):
+    if _is(t, F32, shape, device):
+        return
     _on_gpu(name, t, device)
     if t.dtype != F32 or tuple(t.shape) != shape:
         _fail(f"{name}: expected fp32 {list(shape)}, got {t.dtype} {list(t.shape)}")
@@ -94,8 +100,8 @@ def _rows16(t):
 
 
 def _like(t):
-    """a dense tensor of t's shape (empty_like keeps strides that say nothing, zeros among them, of sizes of one)"""
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    """a dense tensor of t's shape (for a dense t empty_like is the shorter call; the strides that it keeps of sizes of one are never read)"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _ptr(t):
@@ -342,7 +348,7 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
     _on_gpu("k", k, dev)
     _on_gpu("v", v, dev)
     _on_gpu("table", table, dev)
-    if not q.dtype == k.dtype == v.dtype:
+    if not q.dtype is k.dtype is v.dtype:
         _fail(f"q, k, v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     if table.dtype != F32:
         _fail(f"table: expected fp32, got {table.dtype}")
@@ -448,17 +454,17 @@ def _rows_of(t, shape):
 
 def _seam_desc(s, x, f, gate, params):
     """the description of a call, its operands (they have to outlive the launch)"""
-    scale, post_weight, post_bias, pre_weight, pre_bias = params = [None if t is None else _dense16(t) for t in params]
+    params = [None if t is None else _dense16(t) for t in params]
     (x, xs), (f, fs), (gate, gs) = rows = [(None, 0) if t is None else _rows_of(t, s.shape) for t in (x, f, gate)]
-    return NormGateDesc(x.data_ptr(), _ptr(f), _ptr(gate), _ptr(scale), _ptr(post_weight), _ptr(post_bias), _ptr(pre_weight), _ptr(pre_bias), s.rows, xs, fs, gs,
+    return NormGateDesc(x.data_ptr(), _ptr(f), _ptr(gate), *[None if t is None else t.data_ptr() for t in params], s.rows, xs, fs, gs,
                         s.c, s.norm, _DT[x.dtype], s.eps), (rows, params)
 
 
 def _seam_forward(s, x, f, gate, params):
-    dev, dt = x.device, x.dtype
+    dev = x.device
     desc, operands = _seam_desc(s, x, f, gate, params)
-    y = torch.empty(s.shape, dtype=dt, device=dev) if f is not None else None
-    h = torch.empty(s.shape, dtype=dt, device=dev) if params[3] is not None else None
+    y = _like(x) if f is not None else None
+    h = _like(x) if params[3] is not None else None
     guard = _guard(dev)
     try:
         check(lib.im2im_norm_gate_fwd(ctypes.byref(desc), _ptr(y), _ptr(h), torch._C._cuda_getCurrentRawStream(dev.index)), "im2im_norm_gate_fwd")
@@ -488,9 +494,9 @@ class _NormGate(torch.autograd.Function):
         dev, dt, c = x.device, x.dtype, s.c
         dy, dh = (None if t is None else (t if t.dtype == dt else t.to(dt)).contiguous() for t in (dy, dh))
         _, need_x, need_f, need_gate, *need = ctx.needs_input_grad
-        dx = torch.empty(s.shape, dtype=dt, device=dev) if need_x else None
-        df = torch.empty(s.shape, dtype=dt, device=dev) if need_f and f is not None else None
-        dgate = torch.empty(s.shape, dtype=dt, device=dev) if need_gate and gate is not None else None
+        dx = _like(x) if need_x else None
+        df = _like(x) if need_f and f is not None else None
+        dgate = _like(x) if need_gate and gate is not None else None
         want = [n and t is not None for n, t in zip(need, params)]
         wanted = sum(want)
         if wanted and c % 4 == 0:                            # one buffer, each row at 16 bytes
@@ -539,18 +545,19 @@ def _seam(x, f, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm,
         _fail(f"x: expected fp32 or bf16 [..., C], got {x.dtype} {list(x.shape)}")
     if not (isinstance(eps, (int, float)) and 0 < eps < math.inf and ctypes.c_float(eps).value > 0):
         _fail(f"eps must be a positive number, got {eps!r}")
-    c = x.shape[-1]
+    dev, shape = x.device, x.shape
+    c = shape[-1]
     if not 1 <= c <= MAX_NORM_CHANNELS:
         _fail(f"x: 1 to {MAX_NORM_CHANNELS} channels, got {c}")
     for name, t in (("f", f), ("gate", gate)):
         if t is not None:
-            _on_gpu(name, t, x.device)
-            if t.dtype != x.dtype or t.shape != x.shape:
+            if not _is(t, x.dtype, shape, dev):
+                _on_gpu(name, t, dev)
                 _fail(f"{name}: expected {x.dtype} {list(x.shape)} as x, got {t.dtype} {list(t.shape)}")
     params = (scale, post_weight, post_bias, pre_weight, pre_bias)
     for name, t in zip(("scale", "post_weight", "post_bias", "pre_weight", "pre_bias"), params):
         if t is not None:
-            _parameter(name, t, (c,), x.device)
+            _parameter(name, t, (c,), dev)
     if f is None and pre_weight is None:
         _fail("weight is missing")
     if f is not None and post_weight is None:
@@ -560,7 +567,7 @@ def _seam(x, f, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm,
     if pre_bias is not None and pre_weight is None:
         _fail("pre_bias needs pre_weight")
     s = _Seam()
-    s.norm, s.eps, s.c, s.shape, s.rows = _NORM[norm], float(eps), c, tuple(x.shape), x.numel() // c
+    s.norm, s.eps, s.c, s.shape, s.rows = _NORM[norm], float(eps), c, shape, x.numel() // c
     if s.rows == 0:
         y = None if f is None else x + 0 * f
         h = None if pre_weight is None else x * pre_weight.to(x.dtype)
