@@ -68,8 +68,8 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   double* ring = reinterpret_cast<double*>(smem + NBUF * buffer);          // [2 * WAVES][a.ring + 4]: four places in a row may run over the end by three
   __shared__ float red[WAVES];
 
-  const int lin = xcd_band(blockIdx.x, gridDim.x), qt = lin % a.nq, h = lin / a.nq / a.groups, group = lin / a.nq % a.groups;
-  const int slot = group * a.nq + qt;
+  const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.q_splits, item = lin / a.q_splits;
+  const int qt = item % a.nq, h = item / a.nq / a.groups, group = item / a.nq % a.groups, slot = (group * a.q_splits + sp) * a.nq + qt;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31), ic = min(i, i_last);
@@ -120,17 +120,17 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       }
       d += __shfl_xor(d, 32);
       del[m] = m == 0 ? d : -lam * d;
-      if (mine && half == 0 && kw == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
+      if (mine && half == 0 && kw == 0 && sp == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
 #pragma unroll
       for (int n = 0; n < DQ / 32; ++n) acc[m][n] = zero16();
     }
     const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
-    const int tiles = (len + KEYS - 1) / KEYS;
+    const int t0 = sp * a.q_tiles, t1 = min(t0 + a.q_tiles, (len + KEYS - 1) / KEYS);
     const T* kp = static_cast<const T*>(a.k) + b * a.ks[0] + (int64_t)(MAPS * h) * a.ks[2];
     const T* vp = static_cast<const T*>(a.v) + b * a.vs[0] + (int64_t)h * a.vs[2];
     int done = 0;                                                // places (line places from line_shift on) that are written
 
-    Raster keys(0, a.gw);
+    Raster keys(t0 * KEYS, a.gw);
     auto fetch = [&](int t, char* to) {                          // tiles in their order
       const int j0 = t * KEYS, valid = min(len - j0, KEYS);
       const T *k = kp + (int64_t)j0 * a.ks[1], *v = vp + (int64_t)j0 * a.vs[1];
@@ -150,10 +150,14 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (min(code, last) - first);
     };
     __syncthreads();                                             // the image before this one is done with the buffers
-    if (tiles) fetch(0, smem);
-    for (int t = 0; t < tiles; ++t) {
+    if (t0 < t1) fetch(t0, smem);
+    if (BIAS && t0 < t1) {                                       // places in front of this part's keys
+      done = grid_code(t0 * KEYS, a.gw);
+      for (int w = threadIdx.x; w < done; w += 64 * WAVES) put_place(line_out, w + line_shift, 0.0, b == b0);
+    }
+    for (int t = t0; t < t1; ++t) {
       const int base = grid_code(t * KEYS, a.gw), valid = min(len - t * KEYS, KEYS);
-      char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
+      char* at = smem + (NBUF == 2 && ((t - t0) & 1) ? buffer : 0);
       lds_loads_done();
       __syncthreads();
       if (BIAS && done < base) {                                 // a place's thread is the same for every image
@@ -164,7 +168,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
         done = base;
         if (!a.ring_wide) __syncthreads();                       // else the places that this tile adds to are others
       }
-      if (NBUF == 2 && t + 1 < tiles) fetch(t + 1, t & 1 ? smem : smem + buffer);
+      if (NBUF == 2 && t + 1 < t1) fetch(t + 1, (t - t0) & 1 ? smem : smem + buffer);
       const unsigned ring_base = (unsigned)base % size;
       const char *Ks = at, *Vs = at + MAPS * QT;
       const int* kc = reinterpret_cast<const int*>(at + TILES);
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
             for (int n = 0; n < DQ / 32; ++n) acc[m][n] = M::mma(M::template load_t<DQ>(Ks + m * QT, sub * 32, ks, n), df, acc[m][n]);
           }
       }
-      if (NBUF == 1 && t + 1 < tiles) {
+      if (NBUF == 1 && t + 1 < t1) {
         __syncthreads();
         fetch(t + 1, smem);
       }
@@ -268,13 +272,17 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
     if (mine && kw == 0) {
 #pragma unroll
       for (int m = 0; m < MAPS; ++m) {
+        float* part = a.dq_part + ((((int64_t)sp * a.B + b) * a.Lq + i) * a.H * MAPS + MAPS * h + m) * a.d;
         T* dst = static_cast<T*>(a.dq) + b * a.dqs[0] + (int64_t)i * a.dqs[1] + (int64_t)(MAPS * h + m) * a.dqs[2];
 #pragma unroll
         for (int n = 0; n < DQ / 32; ++n)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int c = n * 32 + 8 * g + 4 * half;
-            if (c < a.d)
+            if (c >= a.d) continue;
+            if (KS == 2 && a.q_splits > 1)
+              store4(part + c, acc[m][n][4 * g] * a.scale, acc[m][n][4 * g + 1] * a.scale, acc[m][n][4 * g + 2] * a.scale, acc[m][n][4 * g + 3] * a.scale);
+            else
               store4(dst + c, acc[m][n][4 * g] * a.scale, acc[m][n][4 * g + 1] * a.scale, acc[m][n][4 * g + 2] * a.scale, acc[m][n][4 * g + 3] * a.scale);
           }
       }
@@ -306,7 +314,8 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   if (threadIdx.x < 4 * NBUF)
     *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
-  const int lin = xcd_band(blockIdx.x, gridDim.x), kt = lin % a.nk, h = lin / a.nk / a.B, b = lin / a.nk % a.B, bh = b * a.H + h;
+  const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.k_splits, item = lin / a.k_splits;
+  const int kt = item % a.nk, h = item / a.nk / a.B, b = item / a.nk % a.B, bh = b * a.H + h;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int len = a.lengths ? max(0, min(a.lengths[b], a.Lk)) : a.Lk;
   const int k0 = kt * QR, k_last = min(k0 + QR, a.Lk) - 1;
@@ -331,14 +340,14 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
 
   const T* qp = static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(MAPS * h) * a.qs[2];
   const T* gp = static_cast<const T*>(a.dout) + ((int64_t)b * a.Lq * a.H + h) * a.dv;
-  const int tiles = k0 < len ? (a.Lq + KEYS - 1) / KEYS : 0;
+  const int t0 = sp * a.k_tiles, t1 = k0 < len ? min(t0 + a.k_tiles, (a.Lq + KEYS - 1) / KEYS) : 0;
   const int64_t gstride = (int64_t)a.H * a.dv;
   TileFetch<T, DQ> qt;
   TileFetch<T, DV> gt;
   qt.prepare(a.qs[1]);
   gt.prepare(gstride);
   const bool full = a.d == DQ && a.dv == DV;
-  Raster queries(a.q_start, a.gw);
+  Raster queries(a.q_start + t0 * KEYS, a.gw);
   auto fetch = [&](int t, char* to) {                             // tiles in their order
     const int i0 = t * KEYS, valid = min(a.Lq - i0, KEYS);
     const T *q = qp + (int64_t)i0 * a.qs[1], *g = gp + (int64_t)i0 * gstride;
@@ -363,12 +372,12 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     fetch_window(rows + 2 * MAPS * KEYS + 4, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
     if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (last - min(code, last));   // falls along the row
   };
-  if (tiles) fetch(0, smem);
-  for (int t = 0; t < tiles; ++t) {
-    char* at = smem + (NBUF == 2 && (t & 1) ? buffer : 0);
+  if (t0 < t1) fetch(t0, smem);
+  for (int t = t0; t < t1; ++t) {
+    char* at = smem + (NBUF == 2 && ((t - t0) & 1) ? buffer : 0);
     lds_loads_done();
     __syncthreads();
-    if (NBUF == 2 && t + 1 < tiles) fetch(t + 1, t & 1 ? smem : smem + buffer);
+    if (NBUF == 2 && t + 1 < t1) fetch(t + 1, (t - t0) & 1 ? smem : smem + buffer);
     const char *Qs = at, *Gs = at + MAPS * QT;
     const int* qc = reinterpret_cast<const int*>(at + TILES);
     const float* rows = reinterpret_cast<const float*>(qc + KEYS);
@@ -429,7 +438,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
         }
       }
     }
-    if (NBUF == 1 && t + 1 < tiles) {
+    if (NBUF == 1 && t + 1 < t1) {
       __syncthreads();
       fetch(t + 1, smem);
     }
@@ -457,26 +466,52 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   }
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
+    float* part = a.dk_part + ((((int64_t)sp * a.B + b) * a.Lk + j) * a.H * MAPS + MAPS * h + m) * a.d;
     T* dst = static_cast<T*>(a.dk) + b * a.dks[0] + (int64_t)j * a.dks[1] + (int64_t)(MAPS * h + m) * a.dks[2];
 #pragma unroll
     for (int n = 0; n < DQ / 32; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int c = n * 32 + 8 * g + 4 * half;
-        if (c < a.d) store4(dst + c, dk[m][n][4 * g] * a.scale, dk[m][n][4 * g + 1] * a.scale, dk[m][n][4 * g + 2] * a.scale, dk[m][n][4 * g + 3] * a.scale);
+        if (c >= a.d) continue;
+        if (KS == 2 && a.k_splits > 1)
+          store4(part + c, dk[m][n][4 * g] * a.scale, dk[m][n][4 * g + 1] * a.scale, dk[m][n][4 * g + 2] * a.scale, dk[m][n][4 * g + 3] * a.scale);
+        else
+          store4(dst + c, dk[m][n][4 * g] * a.scale, dk[m][n][4 * g + 1] * a.scale, dk[m][n][4 * g + 2] * a.scale, dk[m][n][4 * g + 3] * a.scale);
       }
   }
+  float* part = a.dv_part + ((((int64_t)sp * a.B + b) * a.Lk + j) * a.H + h) * a.dv;
   T* dst = static_cast<T*>(a.dvv) + b * a.dvs[0] + (int64_t)j * a.dvs[1] + (int64_t)h * a.dvs[2];
 #pragma unroll
   for (int n = 0; n < DV / 32; ++n)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int c = n * 32 + 8 * g + 4 * half;
-      if (c < a.dv) store4(dst + c, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
+      if (c >= a.dv) continue;
+      if (KS == 2 && a.k_splits > 1) store4(part + c, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
+      else store4(dst + c, dv[n][4 * g], dv[n][4 * g + 1], dv[n][4 * g + 2], dv[n][4 * g + 3]);
     }
 }
 
 // ------------------------------------------------------------------------------------------------------ joining the parts
+// dq, dk and dv of split calls: the parts summed in their order, four channels a thread
+struct JoinArgs {
+  const float* part[3];
+  void* out[3];
+  int64_t st[3][3], n[3];    // strides of batch, token and head; elements
+  int splits[3], L[3], heads[3], d[3];
+};
+template <typename T> __global__ __launch_bounds__(256) void attn_join_kernel(const JoinArgs a) {
+  const int w = blockIdx.y;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= a.n[w]) return;
+  f32x4 s = *reinterpret_cast<const f32x4*>(a.part[w] + at);
+  for (int p = 1; p < a.splits[w]; ++p) s += *reinterpret_cast<const f32x4*>(a.part[w] + p * a.n[w] + at);
+  const int c = (int)(at % a.d[w]), head = (int)(at / a.d[w] % a.heads[w]);
+  const int64_t token = at / a.d[w] / a.heads[w];
+  store4(static_cast<T*>(a.out[w]) + token / a.L[w] * a.st[w][0] + token % a.L[w] * a.st[w][1] + head * a.st[w][2] + c, s[0], s[1], s[2], s[3]);
+}
+
 // line[h][x] = sum over the slots whose queries reach x: 64 places a workgroup, the slots dealt to its 16 waves (bound by the latency of these loads:
 // 10 us for 312 slots of 8 x 1521; with four waves 28)
 __global__ __launch_bounds__(1024) void attn_line_sum_kernel(const AttnArgs a, double* sum) {
@@ -489,7 +524,7 @@ __global__ __launch_bounds__(1024) void attn_line_sum_kernel(const AttnArgs a, d
       const int first = grid_code(a.q_start + i0, a.gw), last = grid_code(a.q_start + min(i0 + ROWS / a.ks_q, a.Lq) - 1, a.gw);
       if (x < a.line_off - last || x > grid_code(a.Lk - 1, a.gw) - first + a.line_off) continue;
 #pragma unroll 8
-      for (int g = wave; g < a.groups; g += 16) acc += (double)a.line_part[((int64_t)(g * a.nq + qt) * a.H + h) * a.line_len + x];
+      for (int g = wave; g < a.groups * a.q_splits; g += 16) acc += (double)a.line_part[((int64_t)(g * a.nq + qt) * a.H + h) * a.line_len + x];
     }
   part[wave][l] = acc;
   __syncthreads();
@@ -543,24 +578,38 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 
 // -------------------------------------------------------------------------------------------------------------------- host
 
-static void set_tiles(AttnArgs* a) {
+// Parts of the tiles that a workgroup would take in turn, at least two tiles each, for as many workgroups as the CUs hold at once, where there would be
+// less than one a CU all the same (fp32: 4 x 24x24 x 4 x 2 x 32, 144 workgroups, keys' gradients 57 -> 41 us; 3 x 17x23 x 5 x 40, 105 of them, 39 -> 33 and
+// 44 -> 35 us; 1 x 28x28 x 2 x 128, 26 of them, a whole training call 295 -> 145 us; joining the parts takes 5 to 6)
+static int split(bool small, int64_t items, int64_t tiles, int per_cu) {
+  const int64_t n = std::min<int64_t>(256 * per_cu / items, tiles / 2);
+  return small && n > 1 ? (int)cdiv(tiles, cdiv(tiles, n)) : 1;
+}
+
+static void set_tiles(AttnArgs* a, const im2im_attention_desc* p) {
   // half as many queries (keys) for each workgroup where there would be less than one workgroup a CU (fp32, 3 x 17x23 x 5 x 40: 66 -> 46 and
   // 69 -> 44 us with 60 of them, 39 and 44 by now; with 320, 10 x 20x20 x 8 x 64 bf16, it costs: 39 -> 51 and 26 -> 27 us)
   a->ks_q = (int64_t)a->B * a->H * cdiv(a->Lq, ROWS) < 256 ? 2 : 1;
   a->ks_k = (int64_t)a->B * a->H * cdiv(a->Lk, ROWS) < 256 ? 2 : 1;
   a->nq = (int)cdiv(a->Lq, ROWS / a->ks_q);
   a->nk = (int)cdiv(a->Lk, ROWS / a->ks_k);
+  const bool wide = a->dv > 64;                                   // as the kernels' launch bounds
+  a->q_splits = split(a->ks_q == 2, (int64_t)a->B * a->H * a->nq, cdiv(a->Lk, KEYS), wide || (p->dtype == IM2IM_F32 && p->maps == 2) ? 1 : 2);
+  a->k_splits = split(a->ks_k == 2, (int64_t)a->B * a->H * a->nk, cdiv(a->Lq, KEYS), wide ? 1 : 2);
 }
 
-struct BwdLayout { int64_t delta, part, line, dlam, bytes; };
+struct BwdLayout { int64_t delta, part, line, dlam, dq, dk, dv, bytes; };
 static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   BwdLayout l;
   l.delta = 0;
   l.line = up((int64_t)a.B * a.H * maps * a.Lq * 4);
   l.part = l.line + (table ? up((int64_t)a.H * a.line_len * 8) : 0);
-  l.dlam = l.part + (table ? up((int64_t)a.groups * a.nq * a.H * a.line_len * 4) : 0);
-  l.bytes = l.dlam + up((int64_t)a.groups * a.nq * a.H * 4);
+  l.dlam = l.part + (table ? up((int64_t)a.groups * a.q_splits * a.nq * a.H * a.line_len * 4) : 0);
+  l.dq = l.dlam + up((int64_t)a.groups * a.q_splits * a.nq * a.H * 4);
+  l.dk = l.dq + (a.q_splits > 1 ? up((int64_t)a.q_splits * a.B * a.Lq * a.H * maps * a.d * 4) : 0);
+  l.dv = l.dk + (a.k_splits > 1 ? up((int64_t)a.k_splits * a.B * a.Lk * a.H * maps * a.d * 4) : 0);
+  l.bytes = l.dv + (a.k_splits > 1 ? up((int64_t)a.k_splits * a.B * a.Lk * a.H * a.dv * 4) : 0);
   return l;
 }
 
@@ -568,6 +617,13 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
 // most 256 MiB and the workspace holds it (several add to their line in memory, a read and a wait a tile).
 static BwdLayout set_groups(AttnArgs* a, int maps, bool table, int64_t ws_bytes) {
   int64_t groups = a->B;
+  if (a->q_splits > 1 || a->k_splits > 1) {                       // parts, if the workspace holds them
+    a->groups = a->B;
+    a->group_images = 1;
+    const BwdLayout l = bwd_layout(*a, maps, table);
+    if (l.bytes <= ws_bytes && l.bytes <= 256ll << 20) return l;
+    a->q_splits = a->k_splits = 1;
+  }
   if (table) groups = std::max<int64_t>(1, std::min<int64_t>(groups, (256ll << 20) / ((int64_t)a->H * a->nq * a->line_len * 4)));
   for (a->group_images = (int)cdiv(a->B, groups);; ++a->group_images) {
     a->groups = (int)cdiv(a->B, a->group_images);
@@ -581,7 +637,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int
   const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4) +
                       (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq)), dim3(64 * WAVES), smem, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq * a.q_splits)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_q_kernel");
 }
 
@@ -590,7 +646,7 @@ template <typename T, int DQ, int DV, int MAPS, bool ROW4> static int launch_bwd
   size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
   if (a.ks_k == 2) smem = std::max<size_t>(smem, (size_t)(MAPS * DQ + DV) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk)), dim3(64 * WAVES), smem, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk * a.k_splits)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_kv_kernel");
 }
 
@@ -599,7 +655,22 @@ template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const Attn
   if (a.line_part) rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, true, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, true, false>(a, st);
   else rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, false, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false, false>(a, st);
   if (rc) return rc;
-  return a.row4q ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
+  rc = a.row4q ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
+  if (rc || (a.q_splits == 1 && a.k_splits == 1)) return rc;
+  JoinArgs j = {};
+  int n = 0;
+  const auto add = [&](const float* part, void* out, const int64_t* stride, int splits, int L, int heads, int d) {
+    if (splits == 1) return;
+    j.part[n] = part; j.out[n] = out; j.splits[n] = splits; j.L[n] = L; j.heads[n] = heads; j.d[n] = d;
+    j.n[n] = (int64_t)a.B * L * heads * d;
+    for (int x = 0; x < 3; ++x) j.st[n][x] = stride[x];
+    ++n;
+  };
+  add(a.dq_part, a.dq, a.dqs, a.q_splits, a.Lq, a.H * MAPS, a.d);
+  add(a.dk_part, a.dk, a.dks, a.k_splits, a.Lk, a.H * MAPS, a.d);
+  add(a.dv_part, a.dvv, a.dvs, a.k_splits, a.Lk, a.H, a.dv);
+  hipLaunchKernelGGL(attn_join_kernel<T>, dim3((unsigned)cdiv(std::max(j.n[0], std::max(j.n[1], j.n[2])), 1024), (unsigned)n), dim3(256), 0, st, j);
+  return check_launch("attn_join_kernel");
 }
 
 template <typename T> static int dispatch_bwd(const AttnArgs& a, int maps, hipStream_t st) {
@@ -616,7 +687,7 @@ using namespace im2im;
 extern "C" int64_t im2im_attention_bwd_workspace_bytes(const im2im_attention_desc* p, int32_t want_table) {
   AttnArgs a = {};
   if (attn_check(p, &a)) return -1;
-  set_tiles(&a);
+  set_tiles(&a, p);
   return set_groups(&a, p->maps, want_table != 0, INT64_MAX).bytes;
 }
 
@@ -638,7 +709,7 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   const bool table = g->dtable != nullptr;
   IM2IM_REQUIRE(p->line && (!table || attn_buckets_ok(p->ny, p->nx, p->thr_y, p->thr_x)));
   IM2IM_REQUIRE((int64_t)a.H * a.dv * e * KEYS < (1ll << 31));
-  set_tiles(&a);
+  set_tiles(&a, p);
   const BwdLayout l = set_groups(&a, p->maps, table, ws_bytes);
   IM2IM_REQUIRE(ws && ws_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
   char* w = static_cast<char*>(ws);
@@ -647,6 +718,8 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
   a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
+  a.dq_part = reinterpret_cast<float*>(w + l.dq); a.dk_part = reinterpret_cast<float*>(w + l.dk); a.dv_part = reinterpret_cast<float*>(w + l.dv);
+  a.q_tiles = (int)cdiv(cdiv(p->Lk, KEYS), a.q_splits); a.k_tiles = (int)cdiv(cdiv(p->Lq, KEYS), a.k_splits);
   // a ring of the window and one tile's advance: a tile's places are then none of those that are being written, and one barrier a tile will do.
   // Where LDS does not hold that (grids over 278 wide), the window alone, and a second barrier.
   a.ring = round64(window_floats(p->gh, p->gw) + code_span(KEYS + 1, p->gh, p->gw));
@@ -663,7 +736,7 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   BucketArgs s = {};
   s.line = table ? line : nullptr;
   s.dlam_part = a.dlam_part; s.dtable = g->dtable; s.dlam = g->dlam;
-  s.ny = table ? p->ny : 0; s.nx = table ? p->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.nq;
+  s.ny = table ? p->ny : 0; s.nx = table ? p->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.q_splits * a.nq;
   for (int m = 0; m + 1 < s.ny / 2; ++m) s.thr_y[m] = p->thr_y[m];
   for (int m = 0; m + 1 < s.nx / 2; ++m) s.thr_x[m] = p->thr_x[m];
   hipLaunchKernelGGL(attn_bucket_sum_kernel, dim3((unsigned)(s.ny * s.nx + (p->maps == 2)), (unsigned)a.H), dim3(64), 0, st, s);

@@ -45,6 +45,8 @@ struct AttnArgs {
   float* line_part;                   // [nq * groups][H][line_len] or null
   float* dlam_part;                   // [nq * groups][H]
   int groups, group_images, ring, ring_wide;   // ring: places in one copy of the LDS accumulator
+  int q_splits, q_tiles, k_splits, k_tiles;    // parts of the keys (queries) for the queries' (keys') gradients, tiles in each
+  float *dq_part, *dk_part, *dv_part;          // [splits][B][tokens][heads][channels]
 };
 
 constexpr float LOG2E = 1.4426950408889634f;

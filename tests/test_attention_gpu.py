@@ -107,6 +107,21 @@ def test_small_workspace(grid, maps, d, monkeypatch):
     assert all(torch.equal(full[n], t) for n, t in train(o, grid).items())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,d", [(1, 32), (1, 64), (1, 104), (2, 32), (2, 56)])
+@pytest.mark.parametrize("grid,lq,q_start", [((17, 23), None, 0), ((1, 700), None, 0), ((3, 256), 100, 300), ((3, 256), 1, 767), ((9, 30), 260, 10)])
+def test_few_images(grid, lq, q_start, maps, d, dtype):
+    """so few workgroups that the keys (and queries) are shared out to more of them, whose parts are joined; lengths that end before, at and behind
+    the ends of those parts"""
+    o = operands(maps, dtype, grid, 4, 1, d, (8, 8), lq=lq, seed=41)
+    n = grid[0] * grid[1]
+    for lengths in (None, [0, 1, 128, n], [129, n - 1, 64, 256]):
+        lengths = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        got = train(o, grid, q_start=q_start, lengths=lengths)
+        check(got, reference(o, grid, q_start=q_start, lengths=lengths))
+        assert all(torch.equal(got[k], t) for k, t in train(o, grid, q_start=q_start, lengths=lengths).items())
+
+
 def test_far_apart_rows():
     """offsets that pass 32 bits: tokens 16 MiB apart"""
     grid, step = (1, 300), 1 << 23
