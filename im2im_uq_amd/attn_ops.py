@@ -183,7 +183,7 @@ def _plan(maps, q_shape, k_shape, v_shape, dtype, table_shape, grid, max_distanc
     # one buffer for the bias of every displacement (its begin) and what the backward needs; places in bytes, at 16
     up = lambda n: (4 * n + 15) // 16 * 16  # noqa: E731
     p.lse_at = up(heads * (2 * gh - 1) * (2 * gw - 1))
-    p.map_at = p.lse_at + up(b * heads * maps * lq)
+    p.map_at = p.lse_at + up(2 * b * heads * maps * lq)
     p.save = p.map_at + up(b * heads * lq * maps * d * maps)
     return p
 
@@ -209,7 +209,7 @@ def _describe_qkv(plan, qkv, lam):
 
 
 def _forward(plan, p, dtype, dev, table, keep):
-    """(out, saved) for the description `p` (its line is filled in): `saved` holds the line, log-sums and map results"""
+    """(out, saved) for the description `p` (its line is filled in): `saved` holds the line, the rows' references and log-sums, and map results"""
     out = torch.empty(plan.out_shape, dtype=dtype, device=dev)
     ws = torch.empty(plan.fwd_ws, dtype=torch.uint8, device=dev) if plan.fwd_ws else None
     guard = _guard(dev)

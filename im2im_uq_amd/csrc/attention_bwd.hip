@@ -1,7 +1,7 @@
 // Grid attention, backward.  With P_m the softmax maps, A = P_1 (- lam P_2) and dP = dO V^T:
 //   dV = A^T dO,   dS_1 = P_1 o (dP - D_1),   dS_2 = P_2 o (-lam dP - D_2),   D_m = rowsum(P_m o dP_m) = dO . O_m (times -lam for m = 2),
 //   dQ_m = scale dS_m K_m,   dK_m = scale dS_m^T Q_m,   dbias(j - i) = sum of dS_1 + dS_2,   dlam = -sum P_2 o dP.
-// Two passes, each with its own tile of the scores (computed again from Q, K and the saved log-sums): D, the queries' gradients and the bias
+// Two passes, each with its own tile of the scores (computed again from Q, K and the rows' saved references and log-sums): D, the queries' gradients and the bias
 // in one, the keys' and values' gradients in the other.  No global atomics: every sum has one order.
 #include "attention_common.h"
 
@@ -111,11 +111,12 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
       load_row_frags<T, DQ>(qf[m], static_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)ic * a.qs[1] + (int64_t)(MAPS * h + m) * a.qs[2], mine,
                             a.d, half);
     load_row_frags<T, DV>(gf, static_cast<const T*>(a.dout) + (((int64_t)b * a.Lq + ic) * a.H + h) * a.dv, mine, a.dv, half);
-    float lse[MAPS], del[MAPS];
+    float top[MAPS], lsum[MAPS], del[MAPS];
     f32x16 acc[MAPS][DQ / 32];
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
-      lse[m] = mine ? a.lse[(bh * MAPS + m) * a.Lq + ic] : INFINITY;
+      top[m] = mine ? a.top[(bh * MAPS + m) * a.Lq + ic] : 0.f;
+      lsum[m] = mine ? a.lsum[(bh * MAPS + m) * a.Lq + ic] : INFINITY;
       // D of this lane's query from dO and the saved map result, half a row in each of its two lanes; kept for the other pass
       const float* o = a.osave + ((bh * a.Lq + ic) * MAPS + m) * a.dv;
       float d = 0.f;
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 #pragma unroll
         for (int m = 0; m < MAPS; ++m)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[m][r] = exp2_(fmaf(s[m][r], scale2, bias[r]) - lse[m]);
+          for (int r = 0; r < 16; ++r) s[m][r] = exp2_(fmaf(s[m][r], scale2, bias[r]) - top[m] - lsum[m]);
         if (valid < sub * 32 + 32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
@@ -320,10 +321,10 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // tiles, codes, [2][MAPS][KEYS] log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
-  const size_t buffer = TILES + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
+  // tiles, codes, [3][MAPS][KEYS] references, log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
+  const size_t buffer = TILES + (KEYS + 3 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
   if (threadIdx.x < 4 * NBUF)
-    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 2 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
+    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 3 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.k_splits, item = lin / a.k_splits;
   const int kt = item % a.nk, h = item / a.nk / a.B, b = item / a.nk % a.B, bh = b * a.H + h;
@@ -373,14 +374,13 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     }
     int* codes = reinterpret_cast<int*>(to + TILES);
     float* rows = reinterpret_cast<float*>(codes + KEYS);
-    const int which = wave_index();                              // a wave fetches log-sums (infinite behind the last query: P = 0) or D of a map
-    if (which < 2 * MAPS) {
-      const float* from = which < MAPS ? a.lse : a.delta;
-      load4_to_lds(lane < valid ? from + ((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + lane : attn_fill + (which < MAPS ? 4 : 0), rows + which * KEYS);
+    for (int which = wave_index(); which < 3 * MAPS; which += WAVES) {          // a wave fetches one of them of a map (behind the last query P = 0)
+      const float* from = which < MAPS ? a.top : which < 2 * MAPS ? a.lsum : a.delta;
+      load4_to_lds(lane < valid ? from + ((int64_t)bh * MAPS + which % MAPS) * a.Lq + i0 + lane : attn_fill + (which / MAPS == 1 ? 4 : 0), rows + which * KEYS);
     }
     const int code = queries.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
     queries.next();
-    fetch_window(rows + 2 * MAPS * KEYS + 4, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
+    fetch_window(rows + 3 * MAPS * KEYS + 4, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
     if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (last - min(code, last));   // falls along the row
   };
   if (t0 < t1) fetch(t0, smem);
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     const char *Qs = at, *Gs = at + MAPS * QT;
     const int* qc = reinterpret_cast<const int*>(at + TILES);
     const float* rows = reinterpret_cast<const float*>(qc + KEYS);
-    const unsigned win = window_place(rows + 2 * MAPS * KEYS + 4, koff);
+    const unsigned win = window_place(rows + 3 * MAPS * KEYS + 4, koff);
     const int valid = min(a.Lq - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
       if (START) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 del = *reinterpret_cast<const f32x4*>(rows + KEYS + sub * 32 + 8 * g + 4 * half);
+          const f32x4 del = *reinterpret_cast<const f32x4*>(rows + 2 * KEYS + sub * 32 + 8 * g + 4 * half);
 #pragma unroll
           for (int e = 0; e < 4; ++e) dp[4 * g + e] = -del[e];
         }
@@ -425,13 +425,13 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
           const int i = m * KEYS + sub * 32 + 8 * g + 4 * half;
-          const f32x4 lse = *reinterpret_cast<const f32x4*>(rows + i);
+          const f32x4 top = *reinterpret_cast<const f32x4*>(rows + i), lsum = *reinterpret_cast<const f32x4*>(rows + MAPS * KEYS + i);
           f32x4 del = {0.f, 0.f, 0.f, 0.f};
-          if (!START) del = *reinterpret_cast<const f32x4*>(rows + MAPS * KEYS + i);
+          if (!START) del = *reinterpret_cast<const f32x4*>(rows + 2 * MAPS * KEYS + i);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            const float p = exp2_(fmaf(s[m][r], scale2, bias[r]) - lse[e]);
+            const float p = exp2_(fmaf(s[m][r], scale2, bias[r]) - top[e] - lsum[e]);
             mix[r] = m == 0 ? p : fmaf(-lam, p, mix[r]);
             s[m][r] = p * (START ? dp[r] : m == 0 ? dp[r] - del[e] : fmaf(-lam, dp[r], -del[e]));
           }
@@ -658,7 +658,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int
 
 template <typename T, int DQ, int DV, int MAPS, bool ROW4> static int launch_bwd_kv(const AttnArgs& a, hipStream_t st) {
   auto kern = a.ks_k == 2 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 2> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 1>;
-  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 2 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
+  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 3 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
   if (a.ks_k == 2) smem = std::max<size_t>(smem, (size_t)(MAPS * DQ + DV) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk * a.k_splits)), dim3(64 * WAVES), smem, st, a);
@@ -728,7 +728,7 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   const BwdLayout l = set_groups(&a, p->maps, table, ws_bytes);
   IM2IM_REQUIRE(ws && ws_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
   char* w = static_cast<char*>(ws);
-  a.dout = g->dout; a.lse = const_cast<float*>(g->lse); a.osave = const_cast<float*>(g->map_out); a.delta = reinterpret_cast<float*>(w + l.delta);
+  a.dout = g->dout; a.top = const_cast<float*>(g->lse); a.lsum = a.top + saved_rows(p); a.osave = const_cast<float*>(g->map_out); a.delta = reinterpret_cast<float*>(w + l.delta);
   a.dq = g->dq; a.dk = g->dk; a.dvv = g->dv;
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;

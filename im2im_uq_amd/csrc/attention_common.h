@@ -32,7 +32,9 @@ struct AttnArgs {
   float scale;                        // of the scores
   // forward
   void* out;                          // [B][Lq][H][dv]
-  float* lse;                         // [B*H][MAPS][Lq] (log2 units) or null
+  // a row's reference (its maximum, or up to 2^8 less) and the log2 of its probabilities' sum over that, [B*H][MAPS][Lq] each, or null.  Apart: a
+  // bias of 1e7 is 2^24 times the sum's logarithm, of which one float for both would keep nothing.
+  float *top, *lsum;
   float* osave;                       // [B*H][Lq][MAPS][dv] or null: each map's own result in 32 bits
   float* part;                        // split keys: [splits][B*H*Lq][MAPS][dv]
   float* part_ml;                     //             [splits][B*H*Lq][MAPS][2]
@@ -293,6 +295,8 @@ __device__ __forceinline__ int xcd_band(int id, int total) {
 inline int code_span(int64_t n, int gh, int gw) { return (int)(gh == 1 ? n - 1 : n - 1 + (n - 1 + gw - 1) / gw * (gw - 1)); }
 inline int window_floats(int gh, int gw) { return code_span(ROWS, gh, gw) + code_span(KEYS, gh, gw) + 1; }
 inline int round64(int n) { return (n + 63) / 64 * 64; }
+
+inline int64_t saved_rows(const im2im_attention_desc* p) { return (int64_t)p->B * p->H * p->maps * p->Lq; }
 
 bool attn_buckets_ok(int32_t ny, int32_t nx, const int32_t* thr_y, const int32_t* thr_x);
 int attn_check(const im2im_attention_desc* p, AttnArgs* a);      // validates the description, fills the common fields

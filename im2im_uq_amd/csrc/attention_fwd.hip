@@ -50,6 +50,12 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // lengths, 213 us (590 TFLOP/s; 1.6 rounds of two workgroups a CU, all 256 registers); one query of 4 x 16384 keys x 8 x 2 x 32 30 us (4.4 TB/s).
 constexpr float GROW = 8.f;
 
+// what the backward takes a row's probabilities from: exp2(score - reference - logarithm).  No key at all: +infinity, they come out as zeros.
+__device__ __forceinline__ void save_row(const AttnArgs& a, int64_t at, float top, float sum) {
+  a.top[at] = sum > 0.f ? top : 0.f;
+  a.lsum[at] = sum > 0.f ? __builtin_amdgcn_logf(sum) : INFINITY;
+}
+
 // TOKEN (one query, nothing saved): a key's bias is taken from the table itself, a launch and the line less; a tile's window is its keys in their order.
 template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS, bool TOKEN = false>
 __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
@@ -270,8 +276,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     inv[m] = sum[m] > 0.f ? 1.f / sum[m] : 0.f;                   // no key at all: a row of zeros
-    if (SAVE && half == 0)                                        // +infinity there: the backward's probabilities come out as zeros
-      a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum[m] > 0.f ? mx[m] + __builtin_amdgcn_logf(sum[m]) : INFINITY;
+    if (SAVE && half == 0) save_row(a, ((int64_t)bh * MAPS + m) * a.Lq + i, mx[m], sum[m]);
   }
   const float lam = MAPS == 2 ? a.lam[h] : 0.f;
   T* out = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + i) * a.H + h) * a.dv;
@@ -364,7 +369,7 @@ template <typename T, int MAPS, int G> __global__ __launch_bounds__(256) void at
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     const float inv = sum[m] > 0.f ? 1.f / sum[m] : 0.f;
-    if (a.lse && l == 0) a.lse[((int64_t)bh * MAPS + m) * a.Lq + i] = sum[m] > 0.f ? top[m] + __builtin_amdgcn_logf(sum[m]) : INFINITY;
+    if (a.top && l == 0) save_row(a, ((int64_t)bh * MAPS + m) * a.Lq + i, top[m], sum[m]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       o[m][e] *= inv;
@@ -519,7 +524,8 @@ extern "C" int im2im_attention_fwd(const im2im_attention_desc* p, void* out, flo
   if (int rc = attn_check(p, &a)) return rc;
   IM2IM_REQUIRE(out && (lse != nullptr) == (map_out != nullptr));
   IM2IM_REQUIRE(p->line || !lse);
-  a.out = out; a.lse = lse; a.osave = map_out;
+  a.out = out; a.osave = map_out;
+  if (lse) { a.top = lse; a.lsum = lse + saved_rows(p); }
   if (!p->line) {
     a.table = p->table; a.ny = p->ny; a.nx = p->nx; a.window = KEYS;
     for (int m = 0; m + 1 < p->ny / 2; ++m) a.thr[m] = p->thr_y[m];

@@ -584,7 +584,8 @@ int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, con
  *   keys gives zeros (and zero gradients).  A table entry of -infinity masks its pairs.
  *   line: of im2im_relpos_line.  ny, nx, thr_y, thr_x: the table's; the backward needs them for dtable.  A forward of one query (Lq = 1) that saves
  *   nothing may have line = null and table instead: it takes each key's bias from there.
- *   lse / map_out (both or neither): saved for the backward: lse [B*H][maps][Lq] fp32, map_out [B*H][Lq][maps][D*maps] fp32.
+ *   lse / map_out (both or neither): saved for the backward: lse [2][B*H][maps][Lq] fp32 (a row's reference, then the log2 of its
+ *   sum over that: one float for both loses the sum where biases are large), map_out [B*H][Lq][maps][D*maps] fp32.
  * im2im_attention_bwd: dout [B][Lq][H][D*maps] dense; dq / dk / dv in the types and index order of q / k / v with their own strides; dtable
  *   [ny][nx][H] fp32 or null; dlam [H] fp32 (maps = 2).  Every sum has a fixed order: repeated calls with the same workspace size give the same
  *   bits.  The workspace may be smaller than im2im_attention_bwd_workspace_bytes says, down to what one image at a time needs: then workgroups take

@@ -1,0 +1,48 @@
+"""Grid attention on the GPU with biases over the whole range of their type: values and gradients against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from attention_reference import U16, U32, attention, check
+from test_attention_gpu import DEV, operands, train
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+LOW = torch.finfo(F32).min
+
+# maps, grid, batch, heads, D, lq, q_start: calls of half and whole workgroups, of split keys and queries, of odd widths, of one query
+CALLS = [(1, (20, 20), 2, 2, 32, None, 0), (1, (4, 8), 64, 8, 64, None, 0), (1, (9, 15), 1, 2, 128, None, 0), (1, (64, 64), 1, 2, 32, 1, 2080),
+         (2, (20, 20), 2, 2, 32, None, 0), (2, (5, 7), 64, 8, 64, None, 0), (2, (40, 30), 1, 1, 40, 70, 600)]
+
+
+def swallowed(o, grid, **kw):
+    """reference where finite biases lie so far apart that a score plus its bias is the bias in 32 bits: each entry by its rank, 48 apart (the others' share
+    is 2^-69), and scores of nothing: q as 2^-60 of itself, the keys' gradients as much larger"""
+    rank = torch.searchsorted(o["table"].unique(), o["table"]).float() * 48
+    table = torch.where(o["table"] == -math.inf, o["table"], rank - rank.max())
+    want = attention(o["q"] * 2.0 ** -60, o["k"], o["v"], table, grid, lam=o["lam"], dout=o["dout"], **kw)
+    want["dk"] = tuple(t * 2.0 ** 60 for t in want["dk"])
+    return want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bias", [1.0, -1e6, -1e7, -1e8, -1e9, LOW, 1e7, 1e9, 2e38])
+@pytest.mark.parametrize("maps,grid,b,heads,d,lq,q_start", CALLS)
+def test_a_common_bias_cancels(maps, grid, b, heads, d, lq, q_start, bias, dtype):
+    """every query's probabilities sum to one in the backward too, so that the values' gradients of an image sum to its output gradients (two
+    maps: 1 - lam times); where the bias swallows the scores, every gradient is that of an even softmax"""
+    o = operands(maps, dtype, grid, b, heads, d, (8, 8), lq=lq, seed=1)
+    o["table"].fill_(bias)
+    n = grid[0] * grid[1]
+    lengths = torch.tensor([(n, n // 2 + 1, 1, 0)[x % 4] for x in range(b)], dtype=torch.int32, device=DEV)
+    got = train(o, grid, lengths=lengths, q_start=q_start)
+    dv, dout, lam = got["dv"].double(), o["dout"].double(), 0.0 if maps == 1 else o["lam"].double()[:, None]
+    dout = torch.where(lengths[:, None, None, None] > 0, dout, 0.0)
+    # each dv is rounded once, P for its product (bf16), exponentials, the row's sum and the chains over queries in 32 bits
+    bf16 = dtype == BF16
+    bound = (U16 if bf16 else U32) * dv.abs().sum(1) + ((U16 if bf16 else 0) + (dout.shape[1] + n / 16 + 64) * U32) * (1 + lam) * dout.abs().sum(1)
+    off = (dv.sum(1) - (1 - lam) * dout.sum(1)).abs()
+    assert (off <= bound).all(), float((off / bound.clamp(min=1e-30)).max())
+    if abs(bias) >= 1e9:
+        check(got, swallowed(o, grid, lengths=lengths, q_start=q_start))
