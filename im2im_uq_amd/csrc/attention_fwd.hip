@@ -51,9 +51,10 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 constexpr float GROW = 8.f;
 
 // what the backward takes a row's probabilities from: exp2(score - reference - logarithm).  No key at all: +infinity, they come out as zeros.
+// A sum of NaN is none of these: its row's probabilities are NaN there as they are here.
 __device__ __forceinline__ void save_row(const AttnArgs& a, int64_t at, float top, float sum) {
-  a.top[at] = sum > 0.f ? top : 0.f;
-  a.lsum[at] = sum > 0.f ? __builtin_amdgcn_logf(sum) : INFINITY;
+  a.top[at] = sum == 0.f ? 0.f : top;
+  a.lsum[at] = sum == 0.f ? INFINITY : __builtin_amdgcn_logf(sum);
 }
 
 // TOKEN (one query, nothing saved): a key's bias is taken from the table itself, a launch and the line less; a tile's window is its keys in their order.
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
   float inv[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    inv[m] = sum[m] > 0.f ? 1.f / sum[m] : 0.f;                   // no key at all: a row of zeros
+    inv[m] = sum[m] == 0.f ? 0.f : 1.f / sum[m];                  // no key at all: a row of zeros
     if (SAVE && half == 0) save_row(a, ((int64_t)bh * MAPS + m) * a.Lq + i, mx[m], sum[m]);
   }
   const float lam = MAPS == 2 ? a.lam[h] : 0.f;
@@ -368,7 +369,7 @@ template <typename T, int MAPS, int G> __global__ __launch_bounds__(256) void at
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    const float inv = sum[m] > 0.f ? 1.f / sum[m] : 0.f;
+    const float inv = sum[m] == 0.f ? 0.f : 1.f / sum[m];
     if (a.top && l == 0) save_row(a, ((int64_t)bh * MAPS + m) * a.Lq + i, top[m], sum[m]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

@@ -1,11 +1,11 @@
-"""Grid attention on the GPU with biases over the whole range of their type: values and gradients against 64 bits."""
+"""Grid attention on the GPU with biases over the whole range of their type and with NaN among the keys: values and gradients against 64 bits."""
 import math
 
 import pytest
 import torch
 
 from attention_reference import U16, U32, attention, check
-from test_attention_gpu import DEV, operands, train
+from test_attention_gpu import DEV, call, operands, train
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -46,3 +46,27 @@ def test_a_common_bias_cancels(maps, grid, b, heads, d, lq, q_start, bias, dtype
     assert (off <= bound).all(), float((off / bound.clamp(min=1e-30)).max())
     if abs(bias) >= 1e9:
         check(got, swallowed(o, grid, lengths=lengths, q_start=q_start))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,grid,b,heads,d,lq,q_start", CALLS)
+def test_a_key_of_nan(maps, grid, b, heads, d, lq, q_start, dtype):
+    """a NaN in one key makes its head's probabilities NaN, all of them: no value that comes from them is a number, and nothing else changes"""
+    o = operands(maps, dtype, grid, b, heads, d, (8, 8), lq=lq, seed=2)
+    n = grid[0] * grid[1]
+    length = n - 3
+    lengths = torch.full((b,), length, dtype=torch.int32, device=DEV)
+    want = train(o, grid, lengths=lengths, q_start=q_start)
+    o["k"][0, length // 2, 0, d - 1] = math.nan
+    got = train(o, grid, lengths=lengths, q_start=q_start)
+    assert got["out"][0, :, 0].isnan().all() and got["dq"][0, :, 0].isnan().all()
+    assert got["dk"][0, :length, 0].isnan().all() and got["dv"][0, :length, 0].isnan().all()
+    assert (got["dk"][0, length:, 0] == 0).all() and (got["dv"][0, length:, 0] == 0).all()
+    assert call(o, grid, lengths=lengths, q_start=q_start)[0, :, 0].isnan().all()
+    for name in ("out", "dq", "dk", "dv"):
+        t, w = got[name].clone(), want[name].clone()
+        h = 0 if name in ("out", "dv") or maps == 1 else slice(0, 2)
+        t[0, :, h] = w[0, :, h] = 0
+        assert torch.equal(t, w), name
+    if heads > 1:
+        assert torch.equal(got["dtable"][..., 1:], want["dtable"][..., 1:])
