@@ -249,10 +249,12 @@ __device__ __forceinline__ int lane_bucket(int delta, int n, int thr, int from) 
   return delta > 0 ? b + side : b;
 }
 
-// a table's entry in units of log2.  A finite entry stays finite (the type's lowest value is a large bias; -infinity is a mask).
+// A table's entry in units of log2.  Entries over 2^126 in size would leave the range: from there on they rise half a unit for one, to 2.5e38 at most, which leaves
+// them in their order and room for a score.  (Any two of them are so far apart that the larger takes all, so by how much does not matter.)
 __device__ __forceinline__ float bias_log2(float t) {
-  const float v = t * LOG2E;
-  return v == -INFINITY && t != -INFINITY ? -1.7e38f : v;
+  constexpr float END = 0x1p126f;
+  const float size = fabsf(t);
+  return size <= END || size == INFINITY ? t * LOG2E : copysignf(fmaf(size - END, 0.5f, END * LOG2E), t);
 }
 
 // LDS buffers of tiles: two (the next tile's loads run behind this tile's work, one barrier a tile), one for the widest heads in 32 bits

@@ -569,8 +569,8 @@ int im2im_center_crop_affine(const float* in, float* out, int64_t B, int32_t Hin
  * Relative position bias by buckets: bias(query, key) = table[by(y_key - y_query)][bx(x_key - x_query)][h].  An axis with n buckets (1 or an even
  * number, at most 64) gives n / 2 to the distances <= 0 and n / 2 to those > 0 (n = 1: everything in one); of these n / 2, bucket m holds the
  * distances |d| >= thr[m - 1] (and < thr[m]): thr is a HOST array of n / 2 - 1 ascending numbers (null where that is 0).
- *   im2im_relpos_line: table [ny][nx][H] fp32 -> line [H][im2im_relpos_line_len(gh, gw)] fp32, the bias of every displacement times log2(e):
- *     what the attention entry points read. */
+ *   im2im_relpos_line: table [ny][nx][H] fp32 -> line [H][im2im_relpos_line_len(gh, gw)] fp32, the bias of every displacement times log2(e) (over 2^126 in
+ *     size: pressed into the type's range in their order), what the attention entry points read. */
 int64_t im2im_relpos_line_len(int32_t gh, int32_t gw);
 int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, const int32_t* thr_y, const int32_t* thr_x, int32_t gh,
                       int32_t gw, float* line, im2im_stream_t stream);

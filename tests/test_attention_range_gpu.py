@@ -9,7 +9,7 @@ from test_attention_gpu import DEV, call, operands, train
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
-LOW = torch.finfo(F32).min
+LOW, HIGH = torch.finfo(F32).min, torch.finfo(F32).max
 
 # maps, grid, batch, heads, D, lq, q_start: calls of half and whole workgroups, of split keys and queries, of odd widths, of one query
 CALLS = [(1, (20, 20), 2, 2, 32, None, 0), (1, (4, 8), 64, 8, 64, None, 0), (1, (9, 15), 1, 2, 128, None, 0), (1, (64, 64), 1, 2, 32, 1, 2080),
@@ -17,9 +17,9 @@ CALLS = [(1, (20, 20), 2, 2, 32, None, 0), (1, (4, 8), 64, 8, 64, None, 0), (1, 
 
 
 def swallowed(o, grid, **kw):
-    """reference where finite biases lie so far apart that a score plus its bias is the bias in 32 bits: each entry by its rank, 48 apart (the others' share
-    is 2^-69), and scores of nothing: q as 2^-60 of itself, the keys' gradients as much larger"""
-    rank = torch.searchsorted(o["table"].unique(), o["table"]).float() * 48
+    """reference where finite biases lie so far apart that a score plus its bias is the bias in 32 bits: each entry by its rank, 800 apart (the others'
+    share, e^-800, is nothing in 64 bits either), and scores of nothing: q as 2^-60 of itself, the keys' gradients as much larger"""
+    rank = torch.searchsorted(o["table"].unique(), o["table"]).float() * 800
     table = torch.where(o["table"] == -math.inf, o["table"], rank - rank.max())
     want = attention(o["q"] * 2.0 ** -60, o["k"], o["v"], table, grid, lam=o["lam"], dout=o["dout"], **kw)
     want["dk"] = tuple(t * 2.0 ** 60 for t in want["dk"])
@@ -70,3 +70,16 @@ def test_a_key_of_nan(maps, grid, b, heads, d, lq, q_start, dtype):
         assert torch.equal(t, w), name
     if heads > 1:
         assert torch.equal(got["dtable"][..., 1:], want["dtable"][..., 1:])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,grid,b,heads,d,lq,q_start", CALLS)
+@pytest.mark.parametrize("entries", [(LOW, -2e38, -2.5e38), (HIGH, 2.3e38, 2.4e38, -1e38), (LOW, HIGH, 1e38, 2e38), (LOW, -math.inf, -3e38), (LOW, 1e9, -1e9)])
+def test_the_ends_of_the_range(maps, grid, b, heads, d, lq, q_start, entries, dtype):
+    """table entries of any finite size are ordered as they are: the largest that a row reaches takes it, alone or in even shares"""
+    o = operands(maps, dtype, grid, b, heads, d, (8, 8), lq=lq, seed=3)
+    pick = torch.randint(len(entries), o["table"].shape, generator=torch.Generator().manual_seed(4))
+    o["table"].copy_(torch.tensor(entries)[pick])
+    want = swallowed(o, grid, q_start=q_start)
+    check(train(o, grid, q_start=q_start), want)
+    check({"out": call(o, grid, q_start=q_start)}, want, ("out",))
