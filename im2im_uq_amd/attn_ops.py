@@ -16,6 +16,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import AttentionDesc, AttentionGrads, Im2ImError, NormGateDesc, check, lib
@@ -335,6 +336,12 @@ def _number(name, x):
 
 
 def _needs_grad(*tensors):
+    """whether autograd has a part in the call: a gradient is wanted, or an operand carries a forward-mode tangent (it need not require a gradient), which
+    the autograd functions refuse"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -573,7 +580,7 @@ def _seam(x, f, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm,
         h = None if pre_weight is None else x * pre_weight.to(x.dtype)
         return h if f is None else (y, h)
     tensors = (x, f, gate, *params)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _needs_grad(*tensors):
         got = _NormGate.apply(s, *tensors)
         return got if f is None or pre_weight is not None else (got, None)
     y, h = _seam_forward(s, x, f, gate, params)
