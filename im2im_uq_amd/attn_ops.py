@@ -349,6 +349,11 @@ def _needs_grad(*tensors):
     return False
 
 
+def _nothing(out, needs, *tensors):
+    """an empty result; where a gradient is wanted, one that every operand has a gradient of (zeros, whatever it holds) through"""
+    return sum((out.sum() * t.sum() for t in tensors if t is not None), out).to(out.dtype) if needs else out
+
+
 def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, scale):
     _on_gpu("q", q)
     dev = q.device
@@ -374,8 +379,7 @@ def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, sca
         lengths = lengths.contiguous()
     needs = _needs_grad(q, k, v, table, lam)
     if plan.desc is None:                                    # nothing is asked for
-        out = v.new_empty(plan.out_shape)
-        return out + 0 * q.sum() if needs else out
+        return _nothing(v.new_empty(plan.out_shape), needs, q, k, v, table, lam)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
     if needs:
         return _GridAttention.apply(q, k, v, table, lam, lengths, plan, q_start)
@@ -428,9 +432,10 @@ def grid_self_attention(qkv, heads, table, grid, lam=None, max_distance=64, scal
     plan = _plan(maps, shape, shape, (b, n, heads, d * maps), qkv.dtype, table.shape, grid, _integers("max_distance", max_distance), _number("scale", scale))
     if n != plan.grid[0] * plan.grid[1]:
         _fail(f"{n} tokens are not the grid {grid}")
+    needs = _needs_grad(qkv, table, lam)
     if plan.desc is None:
-        return qkv[..., :c3 // 3]
-    if _needs_grad(qkv, table, lam):
+        return _nothing(qkv.new_empty((b, n, c3 // 3)), needs, qkv, table, lam)
+    if needs:
         return _GridSelfAttention.apply(qkv, table, lam, plan)
     qkv, table, lam = _dense16(qkv), table.contiguous(), None if lam is None else lam.contiguous()
     return _forward(plan, _describe_qkv(plan, qkv, lam), qkv.dtype, qkv.device, table, False)[0].view(b, n, c3 // 3)
@@ -575,12 +580,13 @@ def _seam(x, f, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm,
         _fail("pre_bias needs pre_weight")
     s = _Seam()
     s.norm, s.eps, s.c, s.shape, s.rows = _NORM[norm], float(eps), c, shape, x.numel() // c
-    if s.rows == 0:
-        y = None if f is None else x + 0 * f
-        h = None if pre_weight is None else x * pre_weight.to(x.dtype)
-        return h if f is None else (y, h)
     tensors = (x, f, gate, *params)
-    if _needs_grad(*tensors):
+    needs = _needs_grad(*tensors)
+    if s.rows == 0:
+        y = None if f is None else _nothing(x.new_empty(shape), needs, *tensors[:6])
+        h = None if pre_weight is None else _nothing(x.new_empty(shape), needs, *tensors)
+        return h if f is None else (y, h)
+    if needs:
         got = _NormGate.apply(s, *tensors)
         return got if f is None or pre_weight is not None else (got, None)
     y, h = _seam_forward(s, x, f, gate, params)
