@@ -75,7 +75,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   __shared__ float red[WAVES];
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.q_splits, item = lin / a.q_splits;
-  const int qt = item % a.nq, h = item / a.nq / a.groups, group = item / a.nq % a.groups, slot = (group * a.q_splits + sp) * a.nq + qt;
+  const int qt = a.qt0 + item % a.q_here, h = item / a.q_here / a.groups, group = item / a.q_here % a.groups, slot = group * a.q_splits + sp;
   const int wave = wave_index() / KS, kw = wave_index() % KS, lane = threadIdx.x & 63, half = lane >> 5;
   const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31), ic = min(i, i_last);
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   const float* line = a.line + (int64_t)h * a.line_len;
   const unsigned size = a.ring, copy = size + 4;
   double* my_ring = ring + (wave_index() * 2 + half) * copy;
-  float* line_out = BIAS ? a.line_part + ((int64_t)slot * a.H + h) * a.line_len : nullptr;
+  float* line_out = BIAS ? a.line_part + (((int64_t)slot * a.q_here + item % a.q_here) * a.H + h) * a.line_len : nullptr;
   const int line_shift = a.line_off - code_last, places = grid_code(a.Lk - 1, a.gw) + qspan + 1;
   // the last lane of a run: of queries side by side within 16 lanes
   const bool run_end = (lane & 15) == 15 || (a.q_start + i + 1) % a.gw == 0;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
     __syncthreads();
     if (lane == 0) red[wave_index()] = dlam;
     __syncthreads();
-    if (threadIdx.x == 0) a.dlam_part[(int64_t)slot * a.H + h] = -(red[0] + red[1] + red[2] + red[3]);
+    if (threadIdx.x == 0) a.dlam_part[((int64_t)slot * a.nq + qt) * a.H + h] = -(red[0] + red[1] + red[2] + red[3]);
   }
 }
 
@@ -527,26 +527,26 @@ template <typename T> __global__ __launch_bounds__(256) void attn_join_kernel(co
   store4(static_cast<T*>(a.out[w]) + token / a.L[w] * a.st[w][0] + token % a.L[w] * a.st[w][1] + head * a.st[w][2] + c, s[0], s[1], s[2], s[3]);
 }
 
-// line[h][x] = sum over the slots whose queries reach x: 64 places a workgroup, the slots dealt to its 16 waves (bound by the latency of these loads:
+// line_sum[h][x] = sum over this launch's slots whose queries reach x, added to the launches' before it: 64 places a workgroup, the slots dealt to its 16 waves (bound by the latency of these loads:
 // 10 us for 312 slots of 8 x 1521; with four waves 28)
-__global__ __launch_bounds__(1024) void attn_line_sum_kernel(const AttnArgs a, double* sum) {
+__global__ __launch_bounds__(1024) void attn_line_sum_kernel(const AttnArgs a) {
   __shared__ double part[16][64];
   const int l = threadIdx.x & 63, x = blockIdx.x * 64 + l, h = blockIdx.y, wave = threadIdx.x >> 6;
-  double acc = 0.0;
+  double acc = 0.0, *sum = a.line_sum + (int64_t)h * a.line_len + x;
   if (x < a.line_len)
-    for (int qt = 0; qt < a.nq; ++qt) {
-      const int i0 = qt * (ROWS / a.ks_q);
+    for (int qt = 0; qt < a.q_here; ++qt) {
+      const int i0 = (a.qt0 + qt) * (ROWS / a.ks_q);
       const int first = grid_code(a.q_start + i0, a.gw), last = grid_code(a.q_start + min(i0 + ROWS / a.ks_q, a.Lq) - 1, a.gw);
       if (x < a.line_off - last || x > grid_code(a.Lk - 1, a.gw) - first + a.line_off) continue;
 #pragma unroll 8
-      for (int g = wave; g < a.groups * a.q_splits; g += 16) acc += (double)a.line_part[((int64_t)(g * a.nq + qt) * a.H + h) * a.line_len + x];
+      for (int g = wave; g < a.groups * a.q_splits; g += 16) acc += (double)a.line_part[(((int64_t)g * a.q_here + qt) * a.H + h) * a.line_len + x];
     }
   part[wave][l] = acc;
   __syncthreads();
   if (wave == 0 && x < a.line_len) {
 #pragma unroll
     for (int w = 1; w < 16; ++w) acc += part[w][l];
-    sum[(int64_t)h * a.line_len + x] = acc;
+    *sum = a.qt0 == 0 ? acc : *sum + acc;
   }
 }
 
@@ -620,7 +620,7 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   l.delta = 0;
   l.line = up((int64_t)a.B * a.H * maps * a.Lq * 4);
   l.part = l.line + (table ? up((int64_t)a.H * a.line_len * 8) : 0);
-  l.dlam = l.part + (table ? up((int64_t)a.groups * a.q_splits * a.nq * a.H * a.line_len * 4) : 0);
+  l.dlam = l.part + (table ? up((int64_t)a.groups * a.q_splits * a.q_chunk * a.H * a.line_len * 4) : 0);
   l.dq = l.dlam + up((int64_t)a.groups * a.q_splits * a.nq * a.H * 4);
   l.dk = l.dq + (a.q_splits > 1 ? up((int64_t)a.q_splits * a.B * a.Lq * a.H * maps * a.d * 4) : 0);
   l.dv = l.dk + (a.k_splits > 1 ? up((int64_t)a.k_splits * a.B * a.Lk * a.H * maps * a.d * 4) : 0);
@@ -628,10 +628,13 @@ static BwdLayout bwd_layout(const AttnArgs& a, int maps, bool table) {
   return l;
 }
 
-// Images that one workgroup of the queries' gradients takes in turn: each workgroup writes a line of its own.  One image where that takes at
-// most 256 MiB and the workspace holds it (several add to their line in memory, a read and a wait a tile).
+// Each workgroup of the queries' gradients writes a line of its own, which is as long as four times the tokens: what has to be bounded.  One image a
+// workgroup where that takes at most 256 MiB and the workspace holds it; else several in turn (they add to their line in memory, a read and a wait
+// a tile).  Where one group of all images takes more than 1 GiB, or than the workspace holds, the pass is cut into launches of as many query
+// tiles as fit, whose lines are summed one launch after the other (8 heads: 256x256 tokens in four launches of 1024 workgroups).
 static BwdLayout set_groups(AttnArgs* a, int maps, bool table, int64_t ws_bytes) {
   int64_t groups = a->B;
+  a->q_chunk = a->nq;
   if (a->q_splits > 1 || a->k_splits > 1) {                       // parts, if the workspace holds them
     a->groups = a->B;
     a->group_images = 1;
@@ -643,8 +646,16 @@ static BwdLayout set_groups(AttnArgs* a, int maps, bool table, int64_t ws_bytes)
   for (a->group_images = (int)cdiv(a->B, groups);; ++a->group_images) {
     a->groups = (int)cdiv(a->B, a->group_images);
     const BwdLayout l = bwd_layout(*a, maps, table);
-    if (l.bytes <= ws_bytes || a->groups == 1) return l;
+    if (l.bytes <= ws_bytes && l.dlam - l.part <= 1ll << 30) return l;
+    if (a->groups == 1 && !table) return l;
+    if (a->groups == 1) break;
   }
+  const int64_t tile = (int64_t)a->H * a->line_len * 4;
+  a->q_chunk = 0;
+  const int64_t room = std::min<int64_t>(1ll << 30, ws_bytes - bwd_layout(*a, maps, table).bytes);
+  a->q_chunk = (int)std::max<int64_t>(1, std::min<int64_t>(a->nq, room / 256 * 256 / tile));
+  a->q_chunk = (int)cdiv(a->nq, cdiv(a->nq, a->q_chunk));
+  return bwd_layout(*a, maps, table);
 }
 
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int launch_bwd_q(const AttnArgs& a, hipStream_t st) {
@@ -652,7 +663,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int
   const size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + KEYS * 4 + (size_t)a.window * 4) +
                       (size_t)(BIAS ? 2 * WAVES * (a.ring + 4) : 0) * 8;
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.nq * a.q_splits)), dim3(64 * WAVES), smem, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.groups * a.H * a.q_here * a.q_splits)), dim3(64 * WAVES), smem, st, a);
   return check_launch("attn_bwd_q_kernel");
 }
 
@@ -666,10 +677,16 @@ template <typename T, int DQ, int DV, int MAPS, bool ROW4> static int launch_bwd
 }
 
 template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const AttnArgs& a, hipStream_t st) {
-  int rc;
-  if (a.line_part) rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, true, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, true, false>(a, st);
-  else rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, false, true>(a, st) : launch_bwd_q<T, DQ, DV, MAPS, false, false>(a, st);
-  if (rc) return rc;
+  int rc = IM2IM_OK;
+  for (AttnArgs c = a; c.qt0 < a.nq; c.qt0 += a.q_chunk) {
+    c.q_here = std::min(a.q_chunk, a.nq - c.qt0);
+    if (a.line_part) rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, true, true>(c, st) : launch_bwd_q<T, DQ, DV, MAPS, true, false>(c, st);
+    else rc = a.row4q ? launch_bwd_q<T, DQ, DV, MAPS, false, true>(c, st) : launch_bwd_q<T, DQ, DV, MAPS, false, false>(c, st);
+    if (rc) return rc;
+    if (!a.line_part) continue;
+    hipLaunchKernelGGL(attn_line_sum_kernel, dim3((unsigned)cdiv(a.line_len, 64), (unsigned)a.H), dim3(1024), 0, st, c);
+    if ((rc = check_launch("attn_line_sum_kernel"))) return rc;
+  }
   rc = a.row4q ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
   if (rc || (a.q_splits == 1 && a.k_splits == 1)) return rc;
   JoinArgs j = {};
@@ -732,6 +749,7 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   a.dq = g->dq; a.dk = g->dk; a.dvv = g->dv;
   for (int x = 0; x < 3; ++x) { a.dqs[x] = g->dq_stride[x]; a.dks[x] = g->dk_stride[x]; a.dvs[x] = g->dv_stride[x]; }
   a.line_part = table ? reinterpret_cast<float*>(w + l.part) : nullptr;
+  a.line_sum = reinterpret_cast<double*>(w + l.line);
   a.dlam_part = reinterpret_cast<float*>(w + l.dlam);
   a.dq_part = reinterpret_cast<float*>(w + l.dq); a.dk_part = reinterpret_cast<float*>(w + l.dk); a.dv_part = reinterpret_cast<float*>(w + l.dv);
   a.q_tiles = (int)cdiv(cdiv(p->Lk, KEYS), a.q_splits); a.k_tiles = (int)cdiv(cdiv(p->Lq, KEYS), a.k_splits);
@@ -742,14 +760,9 @@ extern "C" int im2im_attention_bwd(const im2im_attention_desc* p, const im2im_at
   if (!a.ring_wide) a.ring = round64(window_floats(p->gh, p->gw));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (int rc = p->dtype == IM2IM_BF16 ? dispatch_bwd<bf16_t>(a, p->maps, st) : dispatch_bwd<float>(a, p->maps, st)) return rc;
-  double* line = reinterpret_cast<double*>(w + l.line);
-  if (table) {
-    hipLaunchKernelGGL(attn_line_sum_kernel, dim3((unsigned)cdiv(a.line_len, 64), (unsigned)a.H), dim3(1024), 0, st, a, line);
-    if (int rc = check_launch("attn_line_sum_kernel")) return rc;
-  }
   if (!table && p->maps == 1) return IM2IM_OK;
   BucketArgs s = {};
-  s.line = table ? line : nullptr;
+  s.line = table ? a.line_sum : nullptr;
   s.dlam_part = a.dlam_part; s.dtable = g->dtable; s.dlam = g->dlam;
   s.ny = table ? p->ny : 0; s.nx = table ? p->nx : 0; s.H = a.H; s.gh = p->gh; s.gw = p->gw; s.slots = a.groups * a.q_splits * a.nq;
   for (int m = 0; m + 1 < s.ny / 2; ++m) s.thr_y[m] = p->thr_y[m];

@@ -44,8 +44,10 @@ struct AttnArgs {
   float* delta;                       // [B*H][MAPS][Lq]: D
   void *dq, *dk, *dvv;
   int64_t dqs[3], dks[3], dvs[3];
-  float* line_part;                   // [nq * groups][H][line_len] or null
-  float* dlam_part;                   // [nq * groups][H]
+  float* line_part;                   // [groups * q_splits * q_chunk][H][line_len] or null
+  double* line_sum;                   // [H][line_len]
+  float* dlam_part;                   // [groups * q_splits * nq][H]
+  int q_chunk, qt0, q_here;           // query tiles of a launch of the queries' pass at most; this launch's first and how many
   int groups, group_images, ring, ring_wide;   // ring: places in one copy of the LDS accumulator
   int q_splits, q_tiles, k_splits, k_tiles;    // parts of the keys (queries) for the queries' (keys') gradients, tiles in each
   float *dq_part, *dk_part, *dv_part;          // [splits][B][tokens][heads][channels]

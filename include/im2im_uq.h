@@ -588,8 +588,8 @@ int im2im_relpos_line(const float* table, int32_t ny, int32_t nx, int32_t H, con
  *   sum over that: one float for both loses the sum where biases are large), map_out [B*H][Lq][maps][D*maps] fp32.
  * im2im_attention_bwd: dout [B][Lq][H][D*maps] dense; dq / dk / dv in the types and index order of q / k / v with their own strides; dtable
  *   [ny][nx][H] fp32 or null; dlam [H] fp32 (maps = 2).  Every sum has a fixed order: repeated calls with the same workspace size give the same
- *   bits.  The workspace may be smaller than im2im_attention_bwd_workspace_bytes says, down to what one image at a time needs: then workgroups take
- *   several images in turn. */
+ *   bits.  The workspace may be smaller than im2im_attention_bwd_workspace_bytes says: then workgroups take several images in turn, and below what one
+ *   image at a time needs, the queries go in several launches.  dtable's share of it is at most 1 GiB, or one line of all heads where that is more. */
 typedef struct {
   const void *q, *k, *v;
   const float* line;
