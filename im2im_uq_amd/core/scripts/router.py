@@ -29,7 +29,7 @@ from ..models.add_uncertainty import add_uncertainty
 from ..models.trunks.unet import UNet
 from ._wandb import wandb
 from .eval import eval_set_metrics, get_images, get_loss_table
-from .train import train_net
+from .train import network_suffix, train_net
 
 
 def fix_randomness(seed=0):
@@ -60,7 +60,7 @@ def expand_sweep(doc):
 
 def _suffix(params):
     return (params['dataset'] + "_" + params['uncertainty_type'] + "_" + str(params['batch_size']) + "_" + str(params['lr']) + "_"
-            + params['input_normalization'] + "_" + params['output_normalization'].replace('.', '_'))
+            + params['input_normalization'] + "_" + params['output_normalization'].replace('.', '_') + network_suffix(params))
 
 
 def build_dataset(params):

@@ -269,10 +269,17 @@ class GlobalBatchSampler(torch.utils.data.Sampler):
             yield batch[lo:hi]
 
 
+def network_suffix(config):
+    """what the names of a run's files say of its network beside the reference's fields: nothing for the reference's own"""
+    if config.get("attention") is None:
+        return ""
+    return f"_{config['attention']}{config.get('attention_blocks', 1)}"
+
+
 def _ckpt_name(checkpoint_dir, epoch, config):
     return (checkpoint_dir + f'/CP_epoch{epoch}_' + config['dataset'] + "_" + config['uncertainty_type'] + "_"
             + str(config['batch_size']) + "_" + str(config['lr']) + "_" + config['input_normalization'] + "_"
-            + config['output_normalization'].replace('.', '_') + '.pth')
+            + config['output_normalization'].replace('.', '_') + network_suffix(config) + '.pth')
 
 
 def run_validation(net, val_loader, val_dataset, device, global_step, epoch, config):
