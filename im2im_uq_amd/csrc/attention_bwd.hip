@@ -3,6 +3,9 @@
 //   dQ_m = scale dS_m K_m,   dK_m = scale dS_m^T Q_m,   dbias(j - i) = sum of dS_1 + dS_2,   dlam = -sum P_2 o dP.
 // Two passes, each with its own tile of the scores (computed again from Q, K and the rows' saved references and log-sums): D, the queries' gradients and the bias
 // in one, the keys' and values' gradients in the other.  No global atomics: every sum has one order.
+// bf16: dS and P enter the products of dQ, dK and dV as bf16 hi + lo.  A row of dS sums to zero, so of dQ only what the keys differ by is left while the
+// roundings of dS to 8 bits kept all of them: 1.41 to 1.54 times as far from its value as by its own rounding alone, at every head size.  Costs a product
+// more each: 78 x 20x20 x 8 x 64 queries' gradients 159 -> 172 us, keys' 121 -> 145; 8 x 32x32 x 8 x 128 136 -> 149 and 114 -> 140.
 #include "attention_common.h"
 
 namespace im2im {
@@ -47,11 +50,6 @@ template <int N> __device__ __forceinline__ void join_halves(f32x16* acc, float*
     }
 }
 
-// Narrow heads: dS enters the products of dQ and dK as bf16 hi + lo.  A row of dS sums to zero, so of dQ only what the keys differ by is left while the
-// roundings of dS keep all of them: at 8 channels dQ was 1.54 times as far from its value as by its own rounding alone, dK 1.51 times (1.49 at 16, 1.41 to
-// 1.47 from 24 on; hi + lo at 32 channels: 42 -> 46.5 us for 10 x 20x20 x 8 x 2 x 32).
-template <typename T, int DQ> __device__ __forceinline__ bool narrow(int d) { return sizeof(T) == 2 && DQ == 32 && d <= 16; }
-
 // -------------------------------------------------------------------------------------- queries' gradients, bias and lam
 // One workgroup: 128 queries of one head, of `group_images` images in turn, against their keys in tiles of 64.
 // Bias gradient: a pair's place in the line is code(j) - code(i) + off.  Within one instruction 32 lanes have 32 different queries and the
@@ -66,7 +64,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  const bool hilo = narrow<T, DQ>(a.d);
+  constexpr bool HILO = sizeof(T) == 2;
   constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -249,12 +247,12 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
         for (int ks = 0; ks < 32 / M::KC; ++ks)
 #pragma unroll
           for (int m = 0; m < MAPS; ++m) {
-            const Frag df = M::pack(s[m], ks);
+            const Frag df = M::pack(s[m], ks), dr = M::pack_rest(s[m], df, ks);
 #pragma unroll
             for (int n = 0; n < DQ / 32; ++n) {
               const Frag kf = M::template load_t<DQ>(Ks + m * QT, sub * 32, ks, n);
               acc[m][n] = M::mma(kf, df, acc[m][n]);
-              if (hilo) acc[m][n] = M::mma(kf, M::pack_rest(s[m], df, ks), acc[m][n]);
+              if (HILO) acc[m][n] = M::mma(kf, dr, acc[m][n]);
             }
           }
       }
@@ -317,7 +315,7 @@ template <typename T, int DQ, int DV, int MAPS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  const bool hilo = narrow<T, DQ>(a.d);
+  constexpr bool HILO = sizeof(T) == 2;
   constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -438,17 +436,21 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
         }
 #pragma unroll
       for (int ks = 0; ks < 32 / M::KC; ++ks) {
-        const Frag pf = M::pack(mix, ks);
+        const Frag pf = M::pack(mix, ks), pr = M::pack_rest(mix, pf, ks);
 #pragma unroll
-        for (int n = 0; n < DV / 32; ++n) dv[n] = M::mma(M::template load_t<DV>(Gs, sub * 32, ks, n), pf, dv[n]);
+        for (int n = 0; n < DV / 32; ++n) {
+          const Frag gf = M::template load_t<DV>(Gs, sub * 32, ks, n);
+          dv[n] = M::mma(gf, pf, dv[n]);
+          if (HILO) dv[n] = M::mma(gf, pr, dv[n]);
+        }
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
-          const Frag df = M::pack(s[m], ks);
+          const Frag df = M::pack(s[m], ks), dr = M::pack_rest(s[m], df, ks);
 #pragma unroll
           for (int n = 0; n < DQ / 32; ++n) {
             const Frag qf = M::template load_t<DQ>(Qs + m * QT, sub * 32, ks, n);
             dk[m][n] = M::mma(qf, df, dk[m][n]);
-            if (hilo) dk[m][n] = M::mma(qf, M::pack_rest(s[m], df, ks), dk[m][n]);
+            if (HILO) dk[m][n] = M::mma(qf, dr, dk[m][n]);
           }
         }
       }

@@ -40,11 +40,10 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // queries, two waves share 32 and take one half of each tile's keys (joined at the end): for calls that would leave CUs without work.
 // The running maximum follows the scores only where they pass it by more than 2^GROW: until then probabilities up to 2^GROW are as exact in
 // 32 bits and in bf16 as those up to 1, and the accumulators need no rescaling (a handful of times a row).
-// SAVE (training): each map's result leaves in 32 bits too, and the probabilities enter the product as bf16 hi + lo, which makes that
-// result exact to about 2^-18: the backward's row sums D = dO . O are taken from it, and the table's gradient, a 32-bit sum with much
-// cancellation, would carry a rounding of P to bf16 (2^-9) in every D.  Without it, of two maps the first takes hi + lo (lam is mostly below one): their
-// difference is smaller than either, and both maps' roundings left 1.5 times the error of a result rounded once (1.15 so; time at 16 x 40x40 x 4 x 2 x 64
-// with none, the first and both as hi + lo: 168, 216 and 254 us).
+// P enters the product as bf16 hi + lo, 16 bits of it: a result is a sum of terms that cancel, and with P rounded to 8 bits one lay 1.15 (one map) to 1.5
+// (two) times as far from its value as its own rounding, many times that where it is small beside its terms.  Costs the matrix unit a second product
+// (inference 78 x 20x20 x 8 x 64: 77 -> 90 us, 8 x 32x32 x 8 x 128: 57 -> 70; two maps, the second one's added, 16 x 40x40 x 4 x 2 x 64, ragged: 213 -> 246).
+// SAVE (training): each map's result leaves in 32 bits too: the backward's row sums D = dO . O are taken from it.
 // Measured (bf16): training 78 x 20x20 x 8 x 64 80 us (320 TFLOP/s; the vector unit issues in 51 % of the cycles, the matrix unit is busy in 20 %: the
 // exponentials, maxima and packing of 64-wide heads bound it), 8 x 32x32 x 8 x 128 67 us (510 TFLOP/s); two maps at 16 x 40x40 x 4 x 2 x 64, half to full
 // lengths, 213 us (590 TFLOP/s; 1.6 rounds of two workgroups a CU, all 256 registers); one query of 4 x 16384 keys x 8 x 2 x 32 30 us (4.4 TB/s).
@@ -62,7 +61,7 @@ template <typename T, int DQ, int DV, int MAPS, bool SAVE, bool ROW4, int KS, bo
 __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void attn_fwd_kernel(const AttnArgs a) {
   using M = Mma<T>;
   using Frag = typename M::Frag;
-  constexpr int HILO = sizeof(T) == 4 ? 0 : SAVE ? MAPS : MAPS - 1;        // the first so many maps' probabilities as hi + lo
+  constexpr bool HILO = sizeof(T) == 2;
   constexpr int QR = ROWS / KS, NB = DV / 32, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t KT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -201,7 +200,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
         for (int m = 0; m < MAPS; ++m) {
           pf[m] = M::pack(s[m], ks);
-          if (m < HILO) pr[m] = M::pack_rest(s[m], pf[m], ks);
+          if (HILO) pr[m] = M::pack_rest(s[m], pf[m], ks);
         }
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(64 * WAVES, DV * sizeof(T) >= 512 ? 1 : 2) void att
 #pragma unroll
           for (int m = 0; m < MAPS; ++m) {
             o[m][n] = M::mma(vf, pf[m], o[m][n]);
-            if (m < HILO) o[m][n] = M::mma(vf, pr[m], o[m][n]);
+            if (HILO) o[m][n] = M::mma(vf, pr[m], o[m][n]);
           }
         }
       }
