@@ -438,7 +438,8 @@ int attn_check(const im2im_attention_desc* p, AttnArgs* a) {
   a->nk = (int)cdiv(p->Lk, ROWS);
   a->scale = p->scale;
   a->window = round64(window_floats(p->gh, p->gw) + 4);            // a run of four may reach three over the end
-  IM2IM_REQUIRE((int64_t)p->B * p->H * p->Lq < (1ll << 31) && (int64_t)p->B * p->H * a->nk < (1ll << 31) / 64);
+  IM2IM_REQUIRE((int64_t)p->B * p->H * p->Lq < (1ll << 31));
+  IM2IM_REQUIRE((int64_t)p->B * p->H * std::max(cdiv(p->Lq, ROWS), cdiv(p->Lk, ROWS)) < (1ll << 32) / (64 * WAVES));      // work-items of a launch
   return IM2IM_OK;
 }
 

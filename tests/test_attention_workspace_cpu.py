@@ -34,3 +34,17 @@ def test_usual_sizes_are_as_they_were():
     """20x20 at batch 78: one image a workgroup"""
     assert need(20, 20, 8, 64, 78) > 78 * 4 * 8 * 39 * 39 * 4
     assert need(20, 20, 8, 64, 78) < 78 * 4 * 8 * 39 * 39 * 4 + (2 << 20)
+
+
+def test_calls_over_a_launch_are_refused():
+    """2^32 work-items: a batch and its heads of up to 2^24 - 1 workgroups, one token or key each, are described; from there on refused"""
+    def tokens(batch, heads, lq, lk):
+        p = AttentionDesc()
+        for k, v in dict(q=4096, k=4096, v=4096, line=4096, B=batch, Lq=lq, Lk=lk, H=heads, D=8, maps=1, gh=1, gw=512, ny=2, nx=2, scale=1.0).items():
+            setattr(p, k, v)
+        c = heads * 8
+        p.q_stride[:], p.k_stride[:], p.v_stride[:] = (lq * c, c, 8), (lk * c, c, 8), (lk * c, c, 8)
+        return lib.im2im_attention_fwd_workspace_bytes(ctypes.byref(p)), lib.im2im_attention_bwd_workspace_bytes(ctypes.byref(p), 0)
+    assert min(tokens((1 << 21) - 1, 8, 1, 1)) >= 0 and min(tokens((1 << 19) - 1, 8, 1, 512)) >= 0 and min(tokens((1 << 19) - 1, 8, 512, 1)) >= 0
+    for sizes in ((1 << 21, 8, 1, 1), (1 << 19, 8, 1, 512), (1 << 19, 8, 512, 1), (1 << 20, 16, 1, 1)):
+        assert tokens(*sizes) == (-1, -1), sizes
