@@ -163,7 +163,8 @@ template <typename T, int D> __device__ __forceinline__ void load_row_frags(type
 static __device__ const float attn_fill[8] = {0.f, 0.f, 0.f, 0.f, INFINITY, INFINITY, INFINITY, INFINITY};
 // Written as assembly: behind the builtin the compiler waits for every such load before the next transposed LDS read, which is the prefetch
 // lost (the instructions have no result in registers; lds_loads_done() is their wait).  A load into LDS may follow the scalar write of M0 that it reads
-// only after one wait state, which the compiler does not put into inline assembly: the s_nop.  M0 is reserved, so it is no clobber that could be named:
+// only after one wait state, which the compiler does not put into inline assembly: the s_nop.  (Five after a vector instruction's write of a base in scalar
+// registers, v_readfirstlane among them: the s_mov and an s_nop of four.)  M0 is reserved, so it is no clobber that could be named:
 // nothing else in the files that include this may use it (tests/test_lds_dma_cpu.py reads the built library for both).
 __device__ __forceinline__ unsigned lds_address(const void* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -179,7 +180,7 @@ __device__ __forceinline__ void lds_loads_done() { __builtin_amdgcn_s_waitcnt(0x
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 __device__ __forceinline__ void load16_to_lds(const void* base, unsigned offset, const void* to) {       // uniform base, bytes of the lane from there
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(lds_address(to)), "s"(base), "v"(offset) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %2, %1" ::"s"(lds_address(to)), "s"(base), "v"(offset) : "memory");
 }
 
 // KEYS rows of a tile, by the whole workgroup.  A lane's places are the same for every tile: their offsets are kept (64 rows of a tensor are
