@@ -6,7 +6,8 @@ trunk has no attention (core/models/trunks/unet.py:33-46); `UNet(attention=...)`
 
 All operators take and return GPU tensors in fp32 or bf16 with fp32 parameters (as the convolutions do), launch on torch's current stream,
 allocate what they need there, never synchronise, and can be captured into a HIP graph.  Softmax statistics and every sum are 32-bit or
-wider, in one fixed order: a repeated call gives the same bits.
+wider, in one fixed order: a repeated call gives the same bits; a bf16 result is 32-bit arithmetic that is rounded once.  Second derivatives and forward-mode tangents
+are refused.
 """
 from __future__ import annotations
 
@@ -398,7 +399,7 @@ def grid_attention(q, k, v, table, grid, max_distance=64, lengths=None, q_start=
     q_start .. q_start + Lq - 1 (all pixels, a band of them, or a single one).  (1, n): a row of n tokens.
     table [ny, nx, heads] fp32: ny and nx buckets for the two axes (each 1, or an even number up to 64: the lower half for distances
     <= 0, the upper half for those > 0; bucket_thresholds has the borders; from `max_distance` on they share the last one).
-    An entry of -inf masks its pairs.
+    An entry of -inf masks its pairs; every finite one is a bias, the type's lowest and largest among them.
     lengths [B] int32 (on the GPU, clipped to 0 .. Lk): keys from there on take no part, whatever they hold; with none left a
     row gives zeros.  scale: 1 / sqrt(D) unless given.
     Gradients: q, k, v, table."""

@@ -59,7 +59,8 @@ template <int N> __device__ __forceinline__ void join_halves(f32x16* acc, float*
 // ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 226 us at 78 x 20x20 x 8 x 64.  ROW4: four
 // queries' terms of a diagonal are summed from lane to lane first; with that and the tiles' asynchronous loads 226 -> 152 us.
 // Bound by the latency of a wave's own chain (scores, probabilities, dP, dS, diagonals) at two waves a SIMD, which is what the registers allow: there the
-// vector unit issues in 36 % of the cycles, LDS is active in 29 %.  8 x 32x32 x 8 x 128: 125 us.
+// vector unit issues in 39 % of the cycles, the matrix unit is busy in 13 %, LDS in 27 %: 171 us at 78 x 20x20 x 8 x 64 by now.  Heads of 128 channels leave one
+// wave a SIMD: 8 x 32x32 x 8 x 128 145 us.
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
   using M = Mma<T>;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
 
 // ---------------------------------------------------------------------------------------------- keys' and values' gradients
 // One workgroup: 128 keys of one image and head (a wave has 32 of them as its columns), the queries in tiles of 64.  Scores and dP are computed
-// once more (two of its four products): cheaper than writing and reading them.  78 x 20x20 x 8 x 64: 110 us, 465 TFLOP/s with them; at three workgroups a
+// once more (two of its four products): cheaper than writing and reading them.  78 x 20x20 x 8 x 64: 143 us, 355 TFLOP/s with them; at three workgroups a
 // CU it spills and loses what the third gains.
 template <typename T, int DQ, int DV, int MAPS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_kernel(const AttnArgs a) {
@@ -596,7 +597,7 @@ __global__ __launch_bounds__(64) void attn_bucket_sum_kernel(const BucketArgs a)
 // -------------------------------------------------------------------------------------------------------------------- host
 
 // Parts of the tiles that a workgroup would take in turn, at least two tiles each, for as many workgroups as the CUs hold at once, where there would be
-// less than one a CU all the same (fp32: 4 x 24x24 x 4 x 2 x 32, 144 workgroups, keys' gradients 57 -> 41 us; 3 x 17x23 x 5 x 40, 105 of them, 39 -> 33 and
+// less than one a CU all the same (fp32: 4 x 24x24 x 4 x 2 x 32, 144 workgroups, keys' gradients 57 -> 42 us; 3 x 17x23 x 5 x 40, 105 of them, 39 -> 33 and
 // 44 -> 35 us; 1 x 28x28 x 2 x 128, 26 of them, a whole training call 295 -> 145 us; joining the parts takes 5 to 6)
 static int split(bool small, int64_t items, int64_t tiles, int per_cu) {
   const int64_t n = std::min<int64_t>(256 * per_cu / items, tiles / 2);

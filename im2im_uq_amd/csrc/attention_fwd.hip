@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void relpos_line_kernel(const LineArgs a) {
 // SAVE (training): each map's result leaves in 32 bits too: the backward's row sums D = dO . O are taken from it.
 // Measured (bf16): training 78 x 20x20 x 8 x 64 80 us (320 TFLOP/s; the vector unit issues in 51 % of the cycles, the matrix unit is busy in 20 %: the
 // exponentials, maxima and packing of 64-wide heads bound it), 8 x 32x32 x 8 x 128 67 us (510 TFLOP/s); two maps at 16 x 40x40 x 4 x 2 x 64, half to full
-// lengths, 213 us (590 TFLOP/s; 1.6 rounds of two workgroups a CU, all 256 registers); one query of 4 x 16384 keys x 8 x 2 x 32 30 us (4.4 TB/s).
+// lengths, 246 us (510 TFLOP/s; 1.6 rounds of two workgroups a CU, all 256 registers); one query of 4 x 16384 keys x 8 x 2 x 32 32 us (4.2 TB/s).
 constexpr float GROW = 8.f;
 
 // what the backward takes a row's probabilities from: exp2(score - reference - logarithm).  No key at all: +infinity, they come out as zeros.

@@ -7,7 +7,7 @@
 //   ds = sum du a n,  dw_post = sum dn z_f,  db_post = sum dn,  dw_pre = sum dh z_y,  db_pre = sum dh        (a = sigmoid(g), n = N_post(f))
 // Bound by HBM: forward reads x, f, g and writes y, h; backward reads x, f, g, dy, dh (the rows' statistics and y itself in 32 bits are
 // computed again: cheaper than reading them) and writes dx, df, dg.  A row stays in the registers of TPR threads.
-// 31200 x 512 bf16: forward 29 us (5.5 TB/s), backward 62 to 69 us (256 MB at 3.7 to 4.1 TB/s; its few workgroups, which keep the weights' sums in
+// 31200 x 512 bf16: forward 29 us (5.5 TB/s), backward 62 to 70 us (256 MB at 3.7 to 4.1 TB/s; its few workgroups, which keep the weights' sums in
 // registers, have half the forward's waves) and 6 us for the joined sums.
 #include "common.h"
 #include "dtypes.h"
@@ -370,7 +370,7 @@ static int64_t norm_rows_per_block(int C) {
   const int tpr = norm_plan(C).tpr;
   return tpr > 256 ? 1 : 256 / tpr;
 }
-// two workgroups a CU, four where each still has eight rounds of rows: 101 -> 71 us at 31200 x 512 bf16; fewer rounds pay for the longer join
+// two workgroups a CU, four where each still has seven rounds of rows: 101 -> 71 us at 31200 x 512 bf16; fewer rounds pay for the longer join
 // (33 -> 35 us at 4097 x 333 fp32)
 static int64_t bwd_blocks(int64_t rows, int C) {
   const int64_t rounds = cdiv(rows, norm_rows_per_block(C));
