@@ -351,8 +351,8 @@ def _needs_grad(*tensors):
 
 
 def _nothing(out, needs, *tensors):
-    """an empty result; where a gradient is wanted, one that every operand has a gradient of (zeros, whatever it holds) through"""
-    return sum((out.sum() * t.sum() for t in tensors if t is not None), out).to(out.dtype) if needs else out
+    """an empty result; where a gradient is wanted, one that every operand has a gradient of zeros through"""
+    return sum((t[:0].sum() for t in tensors if t is not None), out).to(out.dtype) if needs else out
 
 
 def _attend(maps, q, k, v, lam, table, grid, max_distance, lengths, q_start, scale):
