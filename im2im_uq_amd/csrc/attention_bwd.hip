@@ -79,6 +79,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
   const int i0 = qt * QR, i_last = min(i0 + QR, a.Lq) - 1;
   const int i = i0 + wave * 32 + (lane & 31), ic = min(i, i_last);
   const bool mine = i < a.Lq, busy = i0 + wave * 32 < a.Lq;
+  const bool behind = i0 + wave * 32 + 32 > a.Lq;                      // some columns have no query: their bias, of pairs that are not there, may be NaN
   const int code_last = grid_code(a.q_start + i0 + QR - 1, a.gw);      // of 32 columns for each wave, on behind the last query
   const int aoff = code_last - grid_code(a.q_start + i, a.gw);
   const int qspan = code_last - grid_code(a.q_start + i0, a.gw);
@@ -125,7 +126,7 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
         if (at < a.dv) d = M::dot(gf[c], o + at, d);
       }
       d += __shfl_xor(d, 32);
-      del[m] = m == 0 ? d : -lam * d;
+      del[m] = !mine ? 0.f : m == 0 ? d : -lam * d;
       if (mine && half == 0 && kw == 0 && sp == 0) a.delta[(bh * MAPS + m) * a.Lq + ic] = del[m];
 #pragma unroll
       for (int n = 0; n < DQ / 32; ++n) acc[m][n] = zero16();
@@ -207,6 +208,11 @@ __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof
             if (sub * 32 + mfma_row(r, half) >= valid)
 #pragma unroll
               for (int m = 0; m < MAPS; ++m) s[m][r] = 0.f;
+        }
+        if (behind && !mine) {
+          dp = zero16();
+#pragma unroll
+          for (int m = 0; m < MAPS; ++m) s[m] = zero16();
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -320,10 +326,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
   constexpr int QR = ROWS / KS, NBUF = buffers<T>(MAPS * DQ + DV);
   constexpr size_t QT = tile_bytes<T>(DQ), TILES = tile_bytes<T>(MAPS * DQ + DV);
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  // tiles, codes, [3][MAPS][KEYS] references, log-sums and D, window; four zeros in front of that: behind the last query a run of four reaches there
-  const size_t buffer = TILES + (KEYS + 3 * MAPS * KEYS + 4 + (size_t)a.window) * 4;
-  if (threadIdx.x < 4 * NBUF)
-    *reinterpret_cast<float*>(smem + (threadIdx.x >> 2) * buffer + TILES + (KEYS + 3 * MAPS * KEYS + (threadIdx.x & 3)) * 4) = 0.f;
+  const size_t buffer = TILES + (KEYS + 3 * MAPS * KEYS + (size_t)a.window) * 4;      // tiles, codes, [3][MAPS][KEYS] references, log-sums and D, window
 
   const int lin = xcd_band(blockIdx.x, gridDim.x), sp = lin % a.k_splits, item = lin / a.k_splits;
   const int kt = item % a.nk, h = item / a.nk / a.B, b = item / a.nk % a.B, bh = b * a.H + h;
@@ -379,8 +382,9 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     }
     const int code = queries.code(), first = __builtin_amdgcn_readfirstlane(code), last = __builtin_amdgcn_readlane(code, valid - 1);
     queries.next();
-    fetch_window(rows + 3 * MAPS * KEYS + 4, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
-    if (threadIdx.x < KEYS) codes[threadIdx.x] = 4 * (last - min(code, last));   // falls along the row
+    fetch_window(rows + 3 * MAPS * KEYS, line, a.line_len, code_first - last + a.line_off, last - first + kspan + 1);
+    // falls along the row.  Rows without a query read the last one's bias (ROW4: the last four's): that of a pair which is not there may be NaN.
+    if (threadIdx.x < KEYS) codes[threadIdx.x] = (int)threadIdx.x < valid ? 4 * (last - code) : ROW4 ? 12 : 0;
   };
   if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; ++t) {
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(64 * WAVES, DV >= 128 ? 1 : 2) void attn_bwd_kv_ker
     const char *Qs = at, *Gs = at + MAPS * QT;
     const int* qc = reinterpret_cast<const int*>(at + TILES);
     const float* rows = reinterpret_cast<const float*>(qc + KEYS);
-    const unsigned win = window_place(rows + 3 * MAPS * KEYS + 4, koff);
+    const unsigned win = window_place(rows + 3 * MAPS * KEYS, koff);
     const int valid = min(a.Lq - t * KEYS, KEYS);
     if (busy)
 #pragma unroll 1
@@ -672,7 +676,7 @@ template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4> static int
 
 template <typename T, int DQ, int DV, int MAPS, bool ROW4> static int launch_bwd_kv(const AttnArgs& a, hipStream_t st) {
   auto kern = a.ks_k == 2 ? attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 2> : attn_bwd_kv_kernel<T, DQ, DV, MAPS, ROW4, 1>;
-  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 3 * MAPS * KEYS + 4 + (size_t)a.window) * 4);
+  size_t smem = buffers<T>(MAPS * DQ + DV) * (tile_bytes<T>(MAPS * DQ + DV) + (KEYS + 3 * MAPS * KEYS + (size_t)a.window) * 4);
   if (a.ks_k == 2) smem = std::max<size_t>(smem, (size_t)(MAPS * DQ + DV) * 64 * 4);
   if (int rc = attn_allow_lds(reinterpret_cast<const void*>(kern), smem)) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)a.B * a.H * a.nk * a.k_splits)), dim3(64 * WAVES), smem, st, a);
@@ -690,7 +694,8 @@ template <typename T, int DQ, int DV, int MAPS> static int launch_bwd(const Attn
     hipLaunchKernelGGL(attn_line_sum_kernel, dim3((unsigned)cdiv(a.line_len, 64), (unsigned)a.H), dim3(1024), 0, st, c);
     if ((rc = check_launch("attn_line_sum_kernel"))) return rc;
   }
-  rc = a.row4q ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
+  // queries four by four: whole runs of four only (a band may end within one)
+  rc = a.row4q && a.Lq % 4 == 0 ? launch_bwd_kv<T, DQ, DV, MAPS, true>(a, st) : launch_bwd_kv<T, DQ, DV, MAPS, false>(a, st);
   if (rc || (a.q_splits == 1 && a.k_splits == 1)) return rc;
   JoinArgs j = {};
   int n = 0;

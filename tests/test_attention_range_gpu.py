@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from attention_reference import U16, U32, attention, check
+from attention_reference import U16, U32, attention, axis_bucket, check
 from test_attention_gpu import DEV, call, operands, train
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +83,47 @@ def test_the_ends_of_the_range(maps, grid, b, heads, d, lq, q_start, entries, dt
     want = swallowed(o, grid, q_start=q_start)
     check(train(o, grid, q_start=q_start), want)
     check({"out": call(o, grid, q_start=q_start)}, want, ("out",))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("entry", [math.nan, math.inf])
+@pytest.mark.parametrize("maps,d,grid,b,heads,lq,q_start", [(1, 32, (16, 33), 2, 2, 5, 40), (1, 64, (16, 16), 2, 2, 70, 30), (1, 128, (12, 20), 1, 1, 33, 0),
+                                                            (1, 64, (9, 15), 64, 8, 40, 0), (2, 32, (16, 33), 2, 2, 5, 40), (2, 64, (12, 20), 33, 8, 33, 10)])
+def test_entries_that_no_pair_has(maps, d, grid, b, heads, lq, q_start, entry, dtype):
+    """what the table holds for distances that no query of a band has to any key changes nothing, and has no gradient"""
+    o = operands(maps, dtype, grid, b, heads, d, (16, 32), lq=lq, seed=7)
+    i, j = torch.arange(q_start, q_start + lq, device=DEV), torch.arange(grid[0] * grid[1], device=DEV)
+    row = axis_bucket((j // grid[1])[None] - (i // grid[1])[:, None], 16, 16) * 32 + axis_bucket((j % grid[1])[None] - (i % grid[1])[:, None], 32, 40)
+    free = torch.ones(16 * 32, dtype=torch.bool, device=DEV)
+    free[row.flatten().unique()] = False
+    free = free.view(16, 32)
+    assert free.sum() > 16
+    want = train(o, grid, q_start=q_start, max_distance=(16, 40))
+    out = call(o, grid, q_start=q_start, max_distance=(16, 40))
+    o["table"][free] = entry
+    got = train(o, grid, q_start=q_start, max_distance=(16, 40))
+    assert torch.equal(call(o, grid, q_start=q_start, max_distance=(16, 40)), out)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    assert (got["dtable"][free] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("maps,d,grid,b,heads,lq,q_start", [(1, 64, (16, 16), 2, 2, 70, 30), (1, 64, (9, 15), 64, 8, 40, 0), (2, 32, (16, 33), 2, 2, 5, 40)])
+@pytest.mark.parametrize("name", ["q", "v", "dout"])
+def test_a_last_query_of_nan(name, maps, d, grid, b, heads, lq, q_start, dtype):
+    """NaN in the last query (its gradient, a value of the first head): no bucket that none of the queries reaches has a gradient, no other head has NaN"""
+    o = operands(maps, dtype, grid, b, heads, d, (16, 32), lq=lq, seed=8)
+    i, j = torch.arange(q_start, q_start + lq, device=DEV), torch.arange(grid[0] * grid[1], device=DEV)
+    row = axis_bucket((j // grid[1])[None] - (i // grid[1])[:, None], 16, 16) * 32 + axis_bucket((j % grid[1])[None] - (i % grid[1])[:, None], 32, 40)
+    free = torch.ones(16 * 32, dtype=torch.bool, device=DEV)
+    free[row.flatten().unique()] = False
+    free = free.view(16, 32)
+    want = train(o, grid, q_start=q_start, max_distance=(16, 40))
+    o[name][0, -1, 0] = math.nan
+    got = train(o, grid, q_start=q_start, max_distance=(16, 40))
+    assert got["dtable"][..., 0].isnan().any() and (got["dtable"][free] == 0).all()
+    assert torch.equal(got["dtable"][..., 1:], want["dtable"][..., 1:])
+    if maps == 2:                                            # lam weighs the second map, which the first one's query is no part of
+        assert got["dlam"][0].isnan() if name != "q" else got["dlam"][0] == want["dlam"][0]
+        assert torch.equal(got["dlam"][1:], want["dlam"][1:])
