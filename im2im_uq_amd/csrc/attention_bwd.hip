@@ -59,7 +59,7 @@ template <int N> __device__ __forceinline__ void join_halves(f32x16* acc, float*
 // ds_add_f32 takes 193 cycles for a wave on this part, ds_add_f64 10.5 (ds_read_b32 7 to 10): 833 -> 226 us at 78 x 20x20 x 8 x 64.  ROW4: four
 // queries' terms of a diagonal are summed from lane to lane first; with that and the tiles' asynchronous loads 226 -> 152 us.
 // Bound by the latency of a wave's own chain (scores, probabilities, dP, dS, diagonals) at two waves a SIMD, which is what the registers allow: there the
-// vector unit issues in 39 % of the cycles, the matrix unit is busy in 13 %, LDS in 27 %: 171 us at 78 x 20x20 x 8 x 64 by now.  Heads of 128 channels leave one
+// vector unit issues in 41 % of the cycles, the matrix unit is busy in 13 %, LDS in 26 %: 172 us at 78 x 20x20 x 8 x 64 by now.  Heads of 128 channels leave one
 // wave a SIMD: 8 x 32x32 x 8 x 128 145 us.
 template <typename T, int DQ, int DV, int MAPS, bool BIAS, bool ROW4, int KS>
 __global__ __launch_bounds__(64 * WAVES, MAPS * DV * sizeof(T) >= 512 || (sizeof(T) == 2 && DV == 128) ? 1 : 2) void attn_bwd_q_kernel(const AttnArgs a) {
